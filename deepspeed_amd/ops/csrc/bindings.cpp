@@ -2,12 +2,13 @@
 //
 // Uses torch-ROCm's native HIP stream API (c10::hip) — no CUDA shims.
 
-#include <torch/extension.h>
+#include "bindings.h"
+
 #include <pybind11/numpy.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
 
 #include <tuple>
+
+void bind_packed(pybind11::module_& m);     // bindings_packed.cpp
 
 std::tuple<at::Tensor, int64_t, int64_t, int64_t, bool, int64_t, int64_t>
 step_plan(const pybind11::sequence& slots,
@@ -108,6 +109,13 @@ extern "C" int ds_paged_rows(const void* q, const void* kpool,
                               int n_merges, int any_merge, int nq, int H,
                               int Hkv, int BS, int max_blocks, int splits,
                               float scale, void* stream);
+extern "C" int ds_paged_shaped(const void* q, const void* kpool,
+                               const void* vpool, const int* table,
+                               const int* lens, const float* slopes, void* out,
+                               float* part, float* part_ml, int n, int H,
+                               int Hkv, int BS, int max_blocks, int blocks,
+                               int splits, float scale, float cap,
+                               void* stream);
 extern "C" int ds_rows_linear(const void* x, int layers, const void* const* w,
                               const float* const* scales,
                               const void* const* bias, void* const* out,
@@ -180,41 +188,6 @@ extern "C" void ds_ce_bwd(const void* logits, const long long* labels,
                           long long V, long long ignore_index, void* stream);
 
 namespace {
-
-int dtype_code(const at::Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return 0;
-    case at::kBFloat16: return 1;
-    case at::kHalf: return 2;
-    default:
-      TORCH_CHECK(false, "unsupported dtype ", t.scalar_type());
-  }
-}
-
-void* cur_stream() {
-  return reinterpret_cast<void*>(c10::hip::getCurrentHIPStream().stream());
-}
-
-// A call's tensors lie on one device, the first's, and its kernels run there,
-// whichever device is the current one. Pointers of another device are no error
-// to a kernel: it faults on them or reads what is not its own.
-struct OneDevice {
-  const char* what;
-  const c10::Device device;
-  const c10::DeviceGuard guard;
-  template <typename... Ts>
-  OneDevice(const char* what_, const at::Tensor& first, const Ts&... more)
-      : what(what_), device(first.device()), guard(device) {
-    (check(more), ...);
-  }
-  void check(const at::Tensor& t) const {
-    TORCH_CHECK(t.device() == device, what, ": tensors on different devices, ",
-                device, " and ", t.device());
-  }
-  void check(const c10::optional<at::Tensor>& t) const {
-    if (t.has_value() && t->defined()) check(*t);
-  }
-};
 
 void fused_adam_flat(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v,
                      c10::optional<at::Tensor> p16, double lr, double beta1,
@@ -400,8 +373,10 @@ static void check_pool(const at::Tensor& q, const at::Tensor& kpool,
 
 at::Tensor paged_decode(at::Tensor q, at::Tensor kpool, at::Tensor vpool,
                         at::Tensor block_table, at::Tensor lens,
-                        int64_t splits, double scale) {
-  const OneDevice on("paged_decode", q, kpool, vpool, block_table, lens);
+                        int64_t splits, double scale, double softcap,
+                        c10::optional<at::Tensor> slopes) {
+  const OneDevice on("paged_decode", q, kpool, vpool, block_table, lens,
+                     slopes);
   check_pool(q, kpool, vpool, "paged_decode");
   const int n = q.size(0), H = q.size(1);
   const int Hkv = kpool.size(1), BS = kpool.size(2);
@@ -419,6 +394,24 @@ at::Tensor paged_decode(at::Tensor q, at::Tensor kpool, at::Tensor vpool,
   auto part_ml = at::empty({splits > 1 ? items * Hkv * 16 * 2 : 0}, f32);
   auto o = at::empty_like(q);
   if (n == 0) return o;
+  if (softcap > 0 || slopes.has_value()) {
+    TORCH_CHECK(softcap >= 0 && softcap < 1e30, "paged_decode: softcap");
+    TORCH_CHECK(!slopes.has_value() ||
+                (slopes->scalar_type() == at::kFloat &&
+                 slopes->is_contiguous() && slopes->numel() == H),
+                "paged_decode: alibi_slopes fp32 [H]");
+    TORCH_CHECK(kpool.size(0) > 0 && kpool.size(0) < (1ll << 31) &&
+                items * 256 < (1ll << 32), "paged_decode: size");
+    const int e = ds_paged_shaped(
+        q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(),
+        block_table.data_ptr<int>(), lens.data_ptr<int>(),
+        slopes.has_value() ? slopes->data_ptr<float>() : nullptr, o.data_ptr(),
+        part.data_ptr<float>(), part_ml.data_ptr<float>(), n, H, Hkv, BS,
+        (int)block_table.size(1), (int)kpool.size(0), (int)splits,
+        (float)scale, (float)softcap, cur_stream());
+    TORCH_CHECK(e == 0, "paged_decode: launch failed, hipError_t ", e);
+    return o;
+  }
   const int e = ds_paged_rows(
       q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(),
       block_table.data_ptr<int>(), nullptr, nullptr, nullptr,
@@ -1413,35 +1406,6 @@ at::Tensor groupwise_dequant(at::Tensor q, at::Tensor scales, int64_t numel,
   return out;
 }
 
-// q, o, do [B, S, H, D], k, v [B, S, Hkv, D] with any strides between tokens
-// and heads that keep 16-byte rows: (batch, token, head) strides, in order.
-struct FlashArgs {
-  int B, S, H, Hkv, D;
-  std::vector<long long> strides;
-  FlashArgs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-            double scale) {
-    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() &&
-                q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
-                q.size(3) == k.size(3), "flash: q [B,S,H,D], k/v [B,S,Hkv,D]");
-    B = q.size(0); S = q.size(1); H = q.size(2); D = q.size(3);
-    Hkv = k.size(2);
-    TORCH_CHECK(D == 64 || D == 96 || D == 128, "flash: D of 64, 96 or 128");
-    TORCH_CHECK(Hkv > 0 && H % Hkv == 0, "flash: H a multiple of Hkv");
-    TORCH_CHECK(scale > 0, "flash: scale must be positive");
-    TORCH_CHECK(q.size(1) < (1 << 30) && q.size(0) * (int64_t)H *
-                ((S + 127) / 128) < (1ll << 31), "flash: size");
-  }
-  void add(const at::Tensor& t, const at::Tensor& like) {
-    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 &&
-                t.sizes() == like.sizes() && t.stride(3) == 1 &&
-                ((uintptr_t)t.data_ptr() & 15) == 0 &&
-                t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-                t.stride(2) % 8 == 0 && t.stride(1) >= 0 &&
-                t.stride(1) < (1 << 24), "flash: bf16 GPU, 16-byte rows");
-    for (int d = 0; d < 3; ++d) strides.push_back(t.stride(d));
-  }
-};
-
 std::tuple<at::Tensor, at::Tensor> flash_attn_fwd(
     at::Tensor q, at::Tensor k, at::Tensor v, double scale, bool causal,
     bool with_lse) {
@@ -1530,7 +1494,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(pybind11::init<const std::string&, int64_t, int64_t, int64_t>())
       .def("all_reduce", &ShmComm::all_reduce);
   m.def("paged_decode", &paged_decode,
-        "split-KV decode attention over a paged KV block table");
+        "split-KV decode attention over a paged KV block table",
+        pybind11::arg("q"), pybind11::arg("kpool"), pybind11::arg("vpool"),
+        pybind11::arg("block_table"), pybind11::arg("lens"),
+        pybind11::arg("splits"), pybind11::arg("scale"),
+        pybind11::arg("softcap") = 0.0,
+        pybind11::arg("alibi_slopes") = c10::nullopt);
   m.def("rows_linear", &rows_linear,
         "linear layers of a few rows, bf16 or groupwise int8 weights");
   m.def("tile_linear", &tile_linear, "linear layers of many rows, bf16",
@@ -1648,6 +1617,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("o"), pybind11::arg("dout"), pybind11::arg("lse"),
         pybind11::arg("scale"), pybind11::arg("causal"),
         pybind11::arg("splits") = 0);
+  bind_packed(m);
   pybind11::class_<AioHandle>(m, "AioHandle")
       .def(pybind11::init<int64_t, int>(),
            pybind11::arg("block_size") = 1 << 20,

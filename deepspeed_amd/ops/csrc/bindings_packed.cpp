@@ -1,0 +1,321 @@
+// Python bindings of the operators for packed rows: masked attention, the norms and
+// rotation of queries and keys, log probabilities of tokens.
+
+#include "bindings.h"
+
+#include <tuple>
+
+extern "C" int ds_packed_spans(const void* ids, int wide, const int* prefix,
+                               int* spans, int B, int S, int N, int causal,
+                               void* stream);
+extern "C" int ds_masked_attention(
+    const void* q, const void* k, const void* v, void* out, float* lse,
+    void* rest, const void* dout, void* dq, void* dk, void* dv, float* stat,
+    float* part, int splits, const int* spans, const float* slopes,
+    const long long* strides, int B, int S, int H, int Hkv, int D, int causal,
+    float scale, float cap, void* stream);
+extern "C" int ds_flash_bwd_splits(int B, int S, int H, int Hkv);
+extern "C" int ds_qk_norm_parts(int tokens);
+extern "C" int ds_qk_norm_rope(
+    const void* q, const void* k, void* yq, void* yk, const void* dq,
+    const void* dk, const void* wq, const void* wk, const float* cs,
+    const float* sn, const int* positions, const long long* strides, int B,
+    int S, int H, int Hk, int D, int rotated, int angles, int half, float eps,
+    float plus, int type, float* part, int parts, void* dwq, void* dwk,
+    void* stream);
+extern "C" int ds_logprobs_parts(int rows, long long V, int top);
+extern "C" int ds_logprobs_fwd(const void* x, long long outer_stride,
+                               long long inner_stride, int inner, int type,
+                               const long long* tokens, float* lp, float* ent,
+                               float* stat, float* top_lp, long long* top_ids,
+                               float* sums, void* lists, int rows, long long V,
+                               int parts, int top, long long ignore,
+                               void* stream);
+extern "C" int ds_logprobs_bwd(const void* x, long long outer_stride,
+                               long long inner_stride, int inner, int type,
+                               const long long* tokens, const float* stat,
+                               const float* ent, const float* glp,
+                               const float* gent, void* dx, int rows,
+                               long long V, long long ignore, void* stream);
+
+namespace {
+
+using Opt = c10::optional<at::Tensor>;
+
+// Threads of a launch are counted in 32 bits.
+constexpr int64_t THREADS = 1ll << 32;
+
+void* data(const Opt& t) {
+  return t.has_value() && t->defined() ? t->data_ptr() : nullptr;
+}
+
+at::Tensor packed_spans(at::Tensor ids, Opt prefix, bool causal) {
+  const OneDevice on("packed_rows", ids, prefix);
+  const bool wide = ids.scalar_type() == at::kLong;
+  TORCH_CHECK(ids.is_cuda() && ids.dim() == 2 && ids.is_contiguous() &&
+              (wide || ids.scalar_type() == at::kInt),
+              "packed_rows: document_ids int32 or int64 [B, S]");
+  const int64_t B = ids.size(0), S = ids.size(1);
+  TORCH_CHECK(S < (1 << 30) && B <= 65535, "packed_rows: size");
+  int64_t N = 0;
+  if (data(prefix)) {
+    TORCH_CHECK(prefix->scalar_type() == at::kInt && prefix->dim() == 2 &&
+                prefix->size(0) == B && prefix->is_contiguous() && causal,
+                "packed_rows: prefix_lens int32 [B, N], causal");
+    N = prefix->size(1);
+  }
+  auto spans = at::empty({4, B, S}, ids.options().dtype(at::kInt));
+  if (spans.numel() == 0) return spans;
+  const int e = ds_packed_spans(
+      ids.data_ptr(), wide, static_cast<const int*>(data(prefix)),
+      spans.data_ptr<int>(), (int)B, (int)S, (int)N, causal, cur_stream());
+  TORCH_CHECK(e == 0, "packed_rows: launch failed, hipError_t ", e);
+  return spans;
+}
+
+struct MaskedArgs : FlashArgs {
+  const int* spans = nullptr;
+  const float* slopes = nullptr;
+  MaskedArgs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+             const Opt& spans_, const Opt& slopes_, double scale, double cap)
+      : FlashArgs(q, k, v, scale) {
+    TORCH_CHECK(cap >= 0 && cap < 1e30, "masked_attention: softcap");
+    TORCH_CHECK((int64_t)B * H * ((S + 127) / 128) * 256 < THREADS &&
+                (int64_t)B * S * H * 16 < THREADS, "masked_attention: size");
+    if (data(spans_)) {
+      TORCH_CHECK(spans_->scalar_type() == at::kInt &&
+                  spans_->is_contiguous() && spans_->dim() == 3 &&
+                  spans_->size(0) == 4 && spans_->size(1) == B &&
+                  spans_->size(2) == S, "masked_attention: rows of another batch");
+      spans = spans_->data_ptr<int>();
+    }
+    if (data(slopes_)) {
+      TORCH_CHECK(slopes_->scalar_type() == at::kFloat &&
+                  slopes_->is_contiguous() && slopes_->numel() == H,
+                  "masked_attention: alibi_slopes fp32 [H]");
+      slopes = slopes_->data_ptr<float>();
+    }
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_fwd(
+    at::Tensor q, at::Tensor k, at::Tensor v, Opt spans, Opt slopes,
+    bool causal, double scale, double cap, bool with_rest) {
+  const OneDevice on("masked_attention", q, k, v, spans, slopes);
+  MaskedArgs a(q, k, v, spans, slopes, scale, cap);
+  auto o = at::empty({a.B, a.S, a.H, a.D}, q.options());
+  auto lse = at::empty({a.B, a.H, a.S}, q.options().dtype(at::kFloat));
+  auto rest = at::empty({with_rest ? o.numel() : 0},
+                        q.options().dtype(at::kChar));
+  a.add(q, q); a.add(k, k); a.add(v, k); a.add(o, q);
+  if (q.numel()) {
+    const int e = ds_masked_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+        lse.data_ptr<float>(), with_rest ? rest.data_ptr() : nullptr, nullptr,
+        nullptr, nullptr, nullptr, nullptr, nullptr, 0, a.spans, a.slopes, a.strides.data(), a.B, a.S, a.H, a.Hkv,
+        a.D, causal, (float)scale, (float)cap, cur_stream());
+    TORCH_CHECK(e == 0, "masked_attention: launch failed, hipError_t ", e);
+  }
+  return {o, lse, rest};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_bwd(
+    at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor o, at::Tensor dout,
+    at::Tensor lse, at::Tensor rest, Opt spans, Opt slopes, bool causal,
+    double scale, double cap) {
+  const OneDevice on("masked_attention", q, k, v, o, dout, lse, rest, spans,
+                     slopes);
+  MaskedArgs a(q, k, v, spans, slopes, scale, cap);
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+              lse.numel() == (int64_t)a.B * a.H * a.S &&
+              rest.scalar_type() == at::kChar && rest.is_contiguous() &&
+              rest.numel() == o.numel(), "masked_attention: lse");
+  const int splits = ds_flash_bwd_splits(a.B, a.S, a.H, a.Hkv);
+  auto dq = at::empty({a.B, a.S, a.H, a.D}, q.options());
+  auto dk = at::empty({a.B, a.S, a.Hkv, a.D}, q.options());
+  auto dv = at::empty({a.B, a.S, a.Hkv, a.D}, q.options());
+  auto stat = at::empty({2, lse.numel()}, lse.options());
+  auto part = at::empty({splits > 1 ? 2 * splits * dk.numel() : 0},
+                        lse.options());
+  a.add(q, q); a.add(k, k); a.add(v, k); a.add(o, q); a.add(dout, q);
+  if (q.numel()) {
+    const int e = ds_masked_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+        lse.data_ptr<float>(), rest.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+        dv.data_ptr(), stat.data_ptr<float>(), part.data_ptr<float>(), splits,
+        a.spans, a.slopes, a.strides.data(), a.B, a.S, a.H, a.Hkv, a.D, causal,
+        (float)scale, (float)cap, cur_stream());
+    TORCH_CHECK(e == 0, "masked_attention: launch failed, hipError_t ", e);
+  }
+  return {dq, dk, dv};
+}
+
+// q [B, S, H, D], k [B, S, Hk, D], any strides but one inside a head; with dq and dk
+// the backward: (dq, dk, dwq, dwk) instead of (q, k).
+std::vector<at::Tensor> qk_norm_rope(at::Tensor q, at::Tensor k, at::Tensor wq,
+                                     at::Tensor wk, at::Tensor cs,
+                                     at::Tensor sn, Opt positions, double eps,
+                                     bool half, bool one_plus, Opt dq, Opt dk) {
+  const OneDevice on("qk_norm_rope", q, k, wq, wk, cs, sn, positions, dq, dk);
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 &&
+              q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+              q.size(3) == k.size(3), "qk_norm_rope: q [B, S, H, D], k [B, S, Hk, D]");
+  const int64_t B = q.size(0), S = q.size(1), H = q.size(2), Hk = k.size(2);
+  const int64_t D = q.size(3), tokens = B * S;
+  const int type = dtype_code(q);
+  TORCH_CHECK(D % 2 == 0 && D >= 2 && D <= 512, "qk_norm_rope: even heads up to 512");
+  for (const auto& w : {wq, wk})
+    TORCH_CHECK(w.dim() == 1 && w.size(0) == D && w.is_contiguous() &&
+                w.scalar_type() == q.scalar_type(),
+                "qk_norm_rope: weights [D] of the heads' type");
+  for (const auto& t : {cs, sn})
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 2 &&
+                t.is_contiguous() && t.sizes() == cs.sizes() && t.size(1) >= 1 &&
+                2 * t.size(1) <= D && t.size(0) < (1ll << 31),
+                "qk_norm_rope: tables fp32 [positions, rotated / 2]");
+  if (data(positions)) {
+    TORCH_CHECK(positions->scalar_type() == at::kInt &&
+                positions->is_contiguous() && positions->numel() == tokens,
+                "qk_norm_rope: positions int32, one a token");
+  } else {
+    TORCH_CHECK(S <= cs.size(0), "qk_norm_rope: tables shorter than the rows");
+  }
+  TORCH_CHECK(tokens * 64 < THREADS && H + Hk < (1 << 24), "qk_norm_rope: size");
+  const bool back = data(dq) != nullptr || data(dk) != nullptr;
+  std::vector<long long> strides;
+  auto add = [&](const at::Tensor& t, const at::Tensor& like) {
+    TORCH_CHECK(t.sizes() == like.sizes() && t.stride(3) == 1 &&
+                t.scalar_type() == q.scalar_type(),
+                "qk_norm_rope: heads of one type, unit stride inside them");
+    for (int d = 0; d < 3; ++d) strides.push_back(t.stride(d));
+  };
+  add(q, q); add(k, k);
+  if (back) {
+    TORCH_CHECK(data(dq) && data(dk), "qk_norm_rope: both gradients");
+    add(*dq, q); add(*dk, k);
+  }
+  auto yq = at::empty({B, S, H, D}, q.options());
+  auto yk = at::empty({B, S, Hk, D}, q.options());
+  std::vector<at::Tensor> out = {yq, yk};
+  const int parts = tokens ? ds_qk_norm_parts((int)tokens) : 0;
+  at::Tensor part;
+  if (back) {
+    out.push_back(tokens ? at::empty_like(wq) : at::zeros_like(wq));
+    out.push_back(tokens ? at::empty_like(wk) : at::zeros_like(wk));
+    part = at::empty({parts, 2, D}, q.options().dtype(at::kFloat));
+  }
+  if (tokens == 0 || H + Hk == 0) return out;
+  const int e = ds_qk_norm_rope(
+      q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), data(dq),
+      data(dk), wq.data_ptr(), wk.data_ptr(), cs.data_ptr<float>(),
+      sn.data_ptr<float>(), static_cast<const int*>(data(positions)),
+      strides.data(), (int)B, (int)S, (int)H, (int)Hk, (int)D,
+      (int)(2 * cs.size(1)), (int)cs.size(0), half, (float)eps,
+      one_plus ? 1.f : 0.f, type, back ? part.data_ptr<float>() : nullptr,
+      parts, back ? out[2].data_ptr() : nullptr,
+      back ? out[3].data_ptr() : nullptr, cur_stream());
+  TORCH_CHECK(e == 0, "qk_norm_rope: launch failed, error ", e);
+  return out;
+}
+
+// Logits as rows of two strides: [V], [N, V] or [B, S, V], unit stride inside.
+struct LogitRows {
+  int64_t rows = 1, V, inner = 1, outer_stride = 0, inner_stride = 0;
+  int type;
+  LogitRows(const at::Tensor& x, const at::Tensor& tokens) {
+    const int64_t n = x.dim();
+    TORCH_CHECK(x.is_cuda() && n >= 1 && n <= 3 && x.stride(n - 1) == 1,
+                "token_logprobs: logits [.., V], unit stride inside");
+    V = x.size(n - 1);
+    if (n == 3) {
+      rows = x.size(0) * x.size(1);
+      inner = x.size(1);
+      outer_stride = x.stride(0);
+      inner_stride = x.stride(1);
+    } else if (n == 2) {
+      rows = inner = x.size(0);
+      inner_stride = x.stride(0);
+    }
+    type = dtype_code(x);
+    TORCH_CHECK(tokens.scalar_type() == at::kLong && tokens.is_contiguous() &&
+                tokens.numel() == rows, "token_logprobs: tokens int64, one a row");
+    TORCH_CHECK(V >= 1 && V < (1ll << 31) && rows * 256 < THREADS,
+                "token_logprobs: size");
+  }
+};
+
+std::vector<at::Tensor> logprobs_fwd(at::Tensor x, at::Tensor tokens,
+                                     int64_t top, int64_t ignore) {
+  const OneDevice on("token_logprobs", x, tokens);
+  const LogitRows r(x, tokens);
+  const int parts = ds_logprobs_parts((int)r.rows, r.V, (int)top);
+  TORCH_CHECK(top >= 0 && top <= 32 && top <= r.V && (top == 0 || parts <= 64),
+              "token_logprobs: up to 32 of up to 500000 tokens");
+  TORCH_CHECK(r.rows * (parts + 1) * 256 < THREADS, "token_logprobs: size");
+  const auto f32 = x.options().dtype(at::kFloat);
+  auto lp = at::empty({r.rows}, f32), ent = at::empty({r.rows}, f32);
+  auto stat = at::empty({r.rows, 2}, f32);
+  auto top_lp = at::empty({r.rows, top}, f32);
+  auto ids = at::empty({r.rows, top}, tokens.options());
+  if (r.rows) {
+    // the parts' sums, then on 8 bytes the waves' lists
+    const int64_t of_sums = (r.rows * parts * 3 + 1) / 2 * 2;
+    auto work = at::empty({of_sums + r.rows * parts * 8 * top}, f32);
+    float* sums = work.data_ptr<float>();
+    const int e = ds_logprobs_fwd(
+        x.data_ptr(), r.outer_stride, r.inner_stride, (int)r.inner, r.type,
+        reinterpret_cast<const long long*>(tokens.data_ptr<int64_t>()),
+        lp.data_ptr<float>(), ent.data_ptr<float>(), stat.data_ptr<float>(),
+        top_lp.data_ptr<float>(),
+        reinterpret_cast<long long*>(ids.data_ptr<int64_t>()), sums,
+        sums + of_sums,
+        (int)r.rows, r.V, parts, (int)top, ignore, cur_stream());
+    TORCH_CHECK(e == 0, "token_logprobs: launch failed, hipError_t ", e);
+  }
+  return {lp, ent, stat, top_lp, ids};
+}
+
+at::Tensor logprobs_bwd(at::Tensor x, at::Tensor tokens, at::Tensor stat,
+                        at::Tensor ent, Opt glp, Opt gent, int64_t ignore) {
+  const OneDevice on("token_logprobs", x, tokens, stat, ent, glp, gent);
+  const LogitRows r(x, tokens);
+  for (const auto& g : {glp, gent})
+    if (data(g))
+      TORCH_CHECK(g->scalar_type() == at::kFloat && g->is_contiguous() &&
+                  g->numel() == r.rows, "token_logprobs: gradients fp32, one a row");
+  TORCH_CHECK(stat.numel() == 2 * r.rows && ent.numel() == r.rows,
+              "token_logprobs: saved rows");
+  auto dx = at::empty(x.sizes(), x.options());
+  if (r.rows) {
+    const int e = ds_logprobs_bwd(
+        x.data_ptr(), r.outer_stride, r.inner_stride, (int)r.inner, r.type,
+        reinterpret_cast<const long long*>(tokens.data_ptr<int64_t>()),
+        stat.data_ptr<float>(), ent.data_ptr<float>(),
+        static_cast<const float*>(data(glp)),
+        static_cast<const float*>(data(gent)), dx.data_ptr(), (int)r.rows, r.V,
+        ignore, cur_stream());
+    TORCH_CHECK(e == 0, "token_logprobs: launch failed, hipError_t ", e);
+  }
+  return dx;
+}
+
+}  // namespace
+
+void bind_packed(pybind11::module_& m) {
+  namespace py = pybind11;
+  m.def("packed_spans", &packed_spans,
+        "the keys that each query sees, the queries that see each key");
+  m.def("masked_attn_fwd", &masked_attn_fwd,
+        "attention over packed rows: (o, logsumexp, what o was rounded by)");
+  m.def("masked_attn_bwd", &masked_attn_bwd,
+        "its backward: (dq, dk, dv)");
+  m.def("qk_norm_rope", &qk_norm_rope,
+        "norms and rotation of queries and keys, or their backward",
+        py::arg("q"), py::arg("k"), py::arg("wq"), py::arg("wk"), py::arg("cos"),
+        py::arg("sin"), py::arg("positions"), py::arg("eps"), py::arg("half"),
+        py::arg("one_plus"), py::arg("dq") = c10::nullopt,
+        py::arg("dk") = c10::nullopt);
+  m.def("logprobs_fwd", &logprobs_fwd,
+        "log probabilities, entropy and best tokens of rows of logits");
+  m.def("logprobs_bwd", &logprobs_bwd, "gradient of the logits");
+}

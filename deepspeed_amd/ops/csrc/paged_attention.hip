@@ -61,6 +61,7 @@ constexpr int D = 128;
 constexpr int KT = 32;        // keys a tile
 constexpr int NW = 4;         // waves a workgroup
 constexpr int OSTR = D + 4;   // floats between columns of a merged tile
+constexpr float LOG2E = 1.4426950408889634f;
 
 // runs[j] = {first row, rows, keys including the new ones, offset of the
 // run's blocks in the table}; items[i] = {run, tile of columns, first key,
@@ -79,6 +80,12 @@ struct Args {
   int H, Hkv, BS, max_blocks, splits;
   float c;              // |scale| * log2(e)
   bool flip;            // scale < 0
+  // shaped scores (one row a run): t = cap tanh(s / cap) - slope distance, in units of
+  // log2, and no block of the table outside of the pool's
+  const float* slopes;  // [H] or null
+  float a2, cap;        // 2 log2(e) scale / cap, cap * log2(e), or 0 and 0
+  float sc;             // scale * log2(e)
+  int blocks;
 };
 
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
@@ -102,8 +109,23 @@ template <bool ALIGNED, bool ONCE>
 struct Keys {
   s16x8 k[2][4], v[8];
 
+  // the block of a key; CHECKED: the pool's first, and `lost`, where it has none such
+  template <bool CHECKED>
+  static __device__ __forceinline__ long long block(const Args& a,
+                                                    const int* tab, int key,
+                                                    bool& lost) {
+    int id = tab[key / a.BS];
+    if (CHECKED && (unsigned)id >= (unsigned)a.blocks) {
+      lost = true;
+      id = 0;
+    }
+    return id;
+  }
+
+  template <bool CHECKED>
   __device__ __forceinline__ void load(const Args& a, const int* tab, int id,
-                                       int hkv, int kb, int kv_len, int lane) {
+                                       int hkv, int kb, int kv_len, int lane,
+                                       bool& lost) {
     const int row = lane & 15, g = lane >> 4;
     if (ALIGNED) {
       const long long blk = id;
@@ -124,7 +146,7 @@ struct Keys {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int key = min(kb + 16 * t + row, kv_len - 1);
-        const long long at = (((long long)tab[key / a.BS] * a.Hkv + hkv) *
+        const long long at = ((block<CHECKED>(a, tab, key, lost) * a.Hkv + hkv) *
                                   a.BS + key % a.BS) * D + 8 * g;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
@@ -134,14 +156,17 @@ struct Keys {
       for (int i = 0; i < 8; ++i) {
         const int key = min(kb + 4 * i + g, kv_len - 1);
         v[i] = *(const s16x8*)(a.vpool +
-                               (((long long)tab[key / a.BS] * a.Hkv + hkv) *
-                                    a.BS + key % a.BS) * D + 8 * row);
+                               ((block<CHECKED>(a, tab, key, lost) * a.Hkv +
+                                 hkv) * a.BS + key % a.BS) * D + 8 * row);
       }
     }
   }
 };
 
-template <int NQ, bool ALIGNED>
+// SHAPED: the scores are capped, fall with the distance, or both (no runs). They leave
+// the first product for units of log2 at once and the rest goes on with c = 1. A block
+// of the table that is not in the pool makes its request's row NaN.
+template <int NQ, bool ALIGNED, bool SHAPED>
 __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) float lds[NW][16 * OSTR];
   __shared__ float lds_ml[NW][NQ * 16][2];
@@ -163,6 +188,9 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
     const int j = blockIdx.x / a.splits, s = blockIdx.x % a.splits;
     row0 = j; m = 1; kv_len = a.lens[j]; tab_at = j * a.max_blocks;
     tile = 0; sole = a.splits == 1;
+    if (SHAPED)
+      kv_len = (int)max(0ll, min((long long)kv_len,
+                                 (long long)a.max_blocks * a.BS));
     const int per = ((kv_len + a.splits - 1) / a.splits + KT - 1) / KT * KT;
     key0 = min(kv_len, s * per);
     key1 = min(kv_len, key0 + per);
@@ -182,13 +210,21 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       qf[n][kk] = *(const s16x8*)(qp + kk * 32);
-      if (a.flip)   // a negative scale: the maxima below want c > 0
+      if (!SHAPED && a.flip)   // a negative scale: the maxima below want c > 0
         qf[n][kk] ^= s16x8{-32768, -32768, -32768, -32768,
                            -32768, -32768, -32768, -32768};
     }
     limit[n] = kv_len - m + tok;
   }
   const int low = kv_len - m + (tile * NQ * 16) / G;  // the first column's
+  const float c = SHAPED ? 1.f : a.c;
+  float slope[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+    slope[n] = SHAPED && a.slopes
+                   ? a.slopes[hkv * G + min((tile * NQ + n) * 16 + col,
+                                            ncols - 1) % G] * LOG2E
+                   : 0.f;
 
   float mx[NQ], l[NQ];
   f32x4 acc[NQ][8];
@@ -211,12 +247,18 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
   // Blocks are looked up a tile ahead of the loads from them: a wave has one tile in
   // flight, and waited for the table's entry before each (8 requests of 16000 in 2 and
   // 12 splits 204 / 142 and 95 / 92 us, 32 of 2000 whole 58 / 48).
+  bool lost = false;
   auto find = [&](int k) __attribute__((always_inline)) {
-    return ALIGNED ? tab[min(k, key1 - 1) / a.BS] : 0;
+    int id = ALIGNED ? tab[min(k, key1 - 1) / a.BS] : 0;
+    if (SHAPED && ALIGNED && (unsigned)id >= (unsigned)a.blocks) {
+      lost = true;
+      id = 0;
+    }
+    return id;
   };
   int id = 0;
   if (kb < key1) {
-    x.load(a, tab, find(kb), hkv, kb, kv_len, lane);
+    x.template load<SHAPED>(a, tab, find(kb), hkv, kb, kv_len, lane, lost);
     id = find(kb + NW * KT);
   }
   for (; kb < key1; kb += NW * KT) {
@@ -244,10 +286,29 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
       }
     // the next tile's loads run behind the rest of this one
     if (kb + NW * KT < key1) {
-      x.load(a, tab, id, hkv, kb + NW * KT, kv_len, lane);
+      x.template load<SHAPED>(a, tab, id, hkv, kb + NW * KT, kv_len, lane, lost);
       id = find(kb + 2 * NW * KT);
     }
 
+    if (SHAPED) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const float far = (float)(limit[n] - kb - 4 * g);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float y = s[n][t][r] * a.sc;
+            if (a.cap > 0.f)     // tanh z = 1 - 2 / (e^2z + 1)
+              y = __builtin_fmaf(
+                  -2.f * a.cap,
+                  __builtin_amdgcn_rcpf(
+                      __builtin_amdgcn_exp2f(s[n][t][r] * a.a2) + 1.f),
+                  a.cap);
+            s[n][t][r] = __builtin_fmaf(-slope[n], far - (16 * t + r), y);
+          }
+      }
+    }
     const bool whole = kb + KT <= key1 && kb + KT - 1 <= low;
     s16x8 hi[NQ], lo[NQ];
 #pragma unroll
@@ -265,7 +326,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
       if (__any(mt > mx[n])) {
         const float mn = fmaxf(mx[n], mt);
-        const float alpha = __builtin_amdgcn_exp2f((mx[n] - mn) * a.c);
+        const float alpha = __builtin_amdgcn_exp2f((mx[n] - mn) * c);
         mx[n] = mn;
         l[n] *= alpha;
 #pragma unroll
@@ -273,12 +334,12 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[n][d][r] *= alpha;
       }
-      const float mc = mx[n] * a.c;
+      const float mc = mx[n] * c;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][r], a.c,
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][t][r], c,
                                                           -mc));
           if (!whole && 16 * t + r > last) p = 0.f;
           l[n] += p;
@@ -302,6 +363,11 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
   }
 
   // ---- merge the four waves, one tile of 16 columns at a time
+  const float unit = c;
+  if (SHAPED && __any(lost)) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) l[n] = __builtin_nanf("");
+  }
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     l[n] += __shfl_xor(l[n], 16, 64);
@@ -324,7 +390,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const float al = __builtin_amdgcn_exp2f(
-            (lds_ml[w][n * 16 + c][0] - mg) * a.c);
+            (lds_ml[w][n * 16 + c][0] - mg) * unit);
         lg += lds_ml[w][n * 16 + c][1] * al;
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] += lds[w][c * OSTR + d0 + e] * al;
@@ -789,10 +855,11 @@ int launch_rows(const Args& a, const int2* merges, int n_items, int n_merges,
                           : launch_block<false>(a, n_items, st);
     if (e) return e;
   } else if (aligned) {
-    hipLaunchKernelGGL((rows_kernel<NQ, true>), grid, dim3(NW * 64), 0, st, a);
+    hipLaunchKernelGGL((rows_kernel<NQ, true, false>), grid, dim3(NW * 64), 0,
+                       st, a);
   } else {
-    hipLaunchKernelGGL((rows_kernel<NQ, false>), grid, dim3(NW * 64), 0, st,
-                       a);
+    hipLaunchKernelGGL((rows_kernel<NQ, false, false>), grid, dim3(NW * 64), 0,
+                       st, a);
   }
   if (any_merge)
     hipLaunchKernelGGL((merge_kernel<NQ>), dim3(n_merges, a.Hkv, 4 * NQ),
@@ -842,11 +909,56 @@ extern "C" int ds_paged_rows(const void* q, const void* kpool,
   a.part_ml = part_ml;
   a.H = H; a.Hkv = Hkv; a.BS = BS; a.max_blocks = max_blocks;
   a.splits = splits;
-  a.c = fabsf(scale) * 1.4426950408889634f;
+  a.c = fabsf(scale) * LOG2E;
   a.flip = scale < 0.f;
+  a.slopes = nullptr;
+  a.a2 = a.cap = a.sc = 0.f;
+  a.blocks = 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int2* mg = (const int2*)merges;
   if (nq == 1) return launch_rows<1>(a, mg, n_items, n_merges, any_merge, st);
   if (nq == 2) return launch_rows<2>(a, mg, n_items, n_merges, any_merge, st);
   return launch_rows<8>(a, mg, n_items, n_merges, any_merge, st);
+}
+
+// One row a request of `lens` keys in `splits` parts, the scores shaped by cap (0:
+// none) and slopes (null: none). The pool has `blocks` blocks. Returns a hipError_t.
+extern "C" int ds_paged_shaped(const void* q, const void* kpool,
+                               const void* vpool, const int* table,
+                               const int* lens, const float* slopes, void* out,
+                               float* part, float* part_ml, int n, int H,
+                               int Hkv, int BS, int max_blocks, int blocks,
+                               int splits, float scale, float cap,
+                               void* stream) {
+  Args a;
+  a.q = (const short*)q;
+  a.kpool = (const short*)kpool;
+  a.vpool = (const short*)vpool;
+  a.table = table;
+  a.runs = a.items = nullptr;
+  a.lens = lens;
+  a.out = (short*)out;
+  a.part = part;
+  a.part_ml = part_ml;
+  a.H = H; a.Hkv = Hkv; a.BS = BS; a.max_blocks = max_blocks;
+  a.splits = splits;
+  a.c = 1.f;      // of the merge: the parts' maxima are in units of log2
+  a.flip = false;
+  a.slopes = slopes;
+  a.sc = scale * LOG2E;
+  a.cap = cap * LOG2E;
+  a.a2 = cap > 0.f ? 2.f * LOG2E * scale / cap : 0.f;
+  a.blocks = blocks;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid(n * splits, Hkv);
+  if (BS % KT == 0)
+    hipLaunchKernelGGL((rows_kernel<1, true, true>), grid, dim3(NW * 64), 0, st,
+                       a);
+  else
+    hipLaunchKernelGGL((rows_kernel<1, false, true>), grid, dim3(NW * 64), 0,
+                       st, a);
+  if (splits > 1)
+    hipLaunchKernelGGL((merge_kernel<1>), dim3(n, Hkv, 4), dim3(128), 0, st, a,
+                       (const int2*)nullptr);
+  return (int)hipGetLastError();
 }

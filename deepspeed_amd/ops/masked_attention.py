@@ -1,0 +1,181 @@
+"""Attention over packed rows (csrc/masked_attention.hip), forward and backward:
+several documents beside one another in a row, prefixes that see themselves both
+ways, scores capped by a tanh, a bias that falls with the distance. bf16, heads of 64,
+96 and 128, grouped key heads; the single-token form over the paged pool is
+``paged_attention.paged_decode_attention``."""
+
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from ._loader import get_ext
+from .attention import _rows, _scaled
+from .linear import untransformed
+
+
+@dataclass
+class PackedRows:
+    """What the rows of a packed batch see, made once a batch by ``packed_rows`` and
+    used by every layer. ``spans`` int32 [4, B, S]: the first key that a query sees and
+    the one behind the last, the first query that sees a key and the one behind the
+    last."""
+
+    spans: torch.Tensor
+    causal: bool
+
+
+def _torch_spans(ids, prefix, causal):
+    B, S = ids.shape
+    at = torch.arange(S, device=ids.device).expand(B, S)
+    begins = torch.ones_like(ids, dtype=torch.bool)
+    begins[:, 1:] = ids[:, 1:] != ids[:, :-1]
+    first = torch.where(begins, at, 0).cummax(1).values
+    later = torch.where(begins, at, S).flip(1).cummin(1).values.flip(1)
+    end = torch.full_like(at, S)
+    end[:, :-1] = later[:, 1:]
+    inside = first
+    if prefix is not None:
+        known = (ids >= 0) & (ids < prefix.shape[1])
+        n = prefix.long().gather(1, torch.where(known, ids, 0).long()) \
+            if prefix.shape[1] else torch.zeros_like(at)
+        inside = first + torch.where(known, n, 0).clamp(min=0).minimum(end - first)
+    if causal:
+        spans = [first, torch.maximum(at + 1, inside),
+                 torch.where(at >= inside, at, first), end]
+    else:
+        spans = [first, end, first, end]
+    return torch.stack([torch.where(ids < 0, at, s) for s in spans]).int()
+
+
+def packed_rows(document_ids: torch.Tensor,
+                prefix_lens: Optional[torch.Tensor] = None,
+                causal: bool = True) -> PackedRows:
+    """``document_ids`` [B, S] int32 or int64: a document is a run of one id, and its
+    tokens see that document alone; rows of a negative id (padding) see nothing and
+    are seen by none. ``prefix_lens`` [B, N] (causal only): the first ``prefix_lens[b,
+    d]`` tokens of the documents of id d are seen by all of their document; ids from N
+    on have no prefix."""
+    if document_ids.dim() != 2 or document_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError("packed_rows: document_ids is int32 or int64 [B, S], got "
+                         f"{document_ids.dtype} {tuple(document_ids.shape)}")
+    if prefix_lens is not None:
+        if not causal:
+            raise ValueError("packed_rows: without causal there is no prefix")
+        if prefix_lens.dim() != 2 or prefix_lens.dtype not in (
+                torch.int32, torch.int64) or \
+                prefix_lens.shape[0] != document_ids.shape[0]:
+            raise ValueError("packed_rows: prefix_lens is int32 or int64 [B, N]")
+        if prefix_lens.device != document_ids.device:
+            raise ValueError("packed_rows: tensors on different devices")
+    if document_ids.is_cuda and get_ext() is not None and untransformed():
+        prefix = None if prefix_lens is None else prefix_lens.int().contiguous()
+        spans = get_ext().packed_spans(document_ids.contiguous(), prefix, causal)
+    else:
+        spans = _torch_spans(document_ids, prefix_lens, causal)
+    return PackedRows(spans, causal)
+
+
+def _torch_attention(q, k, v, spans, causal, scale, softcap, slopes):
+    """The formulas on whole score matrices, in fp32 (fp64 for fp64)."""
+    B, S, H, D = q.shape
+    G = H // k.shape[2]
+    wide = torch.float64 if q.dtype is torch.float64 else torch.float32
+    qt, kt, vt = (x.to(wide).transpose(1, 2) for x in (q, k, v))
+    kt, vt = (x.repeat_interleave(G, 1) for x in (kt, vt))
+    t = (qt @ kt.transpose(2, 3).contiguous()) * scale
+    if softcap:
+        t = torch.tanh(t / softcap) * softcap
+    at = torch.arange(S, device=q.device)
+    if slopes is not None:
+        t = t - slopes.to(wide).view(H, 1, 1) * (at[:, None] - at).abs()
+    if spans is not None:
+        lo, hi = (x[:, None, :, None] for x in spans[:2])
+        seen = (at >= lo) & (at < hi)
+    else:
+        seen = at <= at[:, None] if causal else at == at
+    t = t.masked_fill(~seen, -math.inf)
+    top = t.amax(-1, keepdim=True).detach()
+    p = torch.exp(t - torch.where(seen.any(-1, keepdim=True), top, 0.0))
+    p = torch.where(seen, p, 0.0)
+    p = p / torch.where(seen.any(-1, keepdim=True), p.sum(-1, keepdim=True), 1.0)
+    return (p @ vt).transpose(1, 2).to(q.dtype)
+
+
+class _MaskedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, spans, slopes, causal, scale, softcap):
+        q, scale, ctx.factor = _scaled(q, scale)
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        o, lse, rest = get_ext().masked_attn_fwd(
+            q, k, v, spans, slopes, causal, scale, softcap,
+            any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, o, lse, rest, spans, slopes)
+        ctx.causal, ctx.scale, ctx.softcap = causal, scale, softcap
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, rest, spans, slopes = ctx.saved_tensors
+        dq, dk, dv = get_ext().masked_attn_bwd(
+            q, k, v, o, _rows(do), lse, rest, spans, slopes, ctx.causal, ctx.scale,
+            ctx.softcap)
+        dq = dq if ctx.factor == 1 else dq * ctx.factor
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _checked_slopes(alibi_slopes, q, what):
+    if alibi_slopes is None:
+        return None
+    if alibi_slopes.requires_grad:
+        raise ValueError(f"{what}: alibi_slopes have no gradient")
+    if alibi_slopes.shape != (q.shape[-2],) or \
+            not alibi_slopes.dtype.is_floating_point:
+        raise ValueError(f"{what}: alibi_slopes is one number a query head, got "
+                         f"{alibi_slopes.dtype} {tuple(alibi_slopes.shape)}")
+    if alibi_slopes.device != q.device:
+        raise ValueError(f"{what}: tensors on different devices")
+    return alibi_slopes.float().contiguous()
+
+
+def _checked_cap(softcap, what):
+    softcap = float(softcap or 0.0)
+    if not 0.0 <= softcap < 1e30:
+        raise ValueError(f"{what}: softcap is 0 (none) or positive, got {softcap}")
+    return softcap
+
+
+def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                     rows: Optional[PackedRows] = None, causal: bool = True,
+                     scale: Optional[float] = None, softcap: float = 0.0,
+                     alibi_slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [B, S, H, D], k and v [B, S, Hkv, D] -> [B, S, H, D], differentiable in q, k
+    and v (once). Scores ``scale q k`` (default 1 / sqrt(D)), with ``softcap`` c
+    then c tanh(score / c), with ``alibi_slopes`` [H] less slope times the distance of
+    query and key, softmax over the keys that a query sees: those of ``rows``, or
+    without them by ``causal`` all up to its own or all there are. A query that sees
+    none gives 0 and has no gradient. On a GPU bf16 and heads of 64, 96 or 128."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or \
+            q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or \
+            k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError("masked_attention: q is [B, S, H, D], k and v are [B, S, Hkv, "
+                         "D] with H a multiple of Hkv, got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if not q.dtype == k.dtype == v.dtype:
+        raise ValueError("masked_attention: q, k and v of one type")
+    if rows is not None and (rows.spans.shape[1:] != q.shape[:2]
+                             or rows.spans.device != q.device):
+        raise ValueError("masked_attention: rows of another batch or device: "
+                         f"{tuple(rows.spans.shape)} for q {tuple(q.shape)}")
+    softcap = _checked_cap(softcap, "masked_attention")
+    slopes = _checked_slopes(alibi_slopes, q, "masked_attention")
+    spans, causal = (rows.spans, rows.causal) if rows is not None else (None, causal)
+    if not q.is_cuda or get_ext() is None or not untransformed():
+        scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[3])
+        return _torch_attention(q, k, v, spans, causal, scale, softcap, slopes)
+    if q.dtype is not torch.bfloat16 or q.shape[3] not in (64, 96, 128):
+        raise ValueError("masked_attention: bf16 and heads of 64, 96 or 128 on a GPU, "
+                         f"got {q.dtype} and {q.shape[3]}")
+    return _MaskedAttentionFn.apply(q, k, v, spans, slopes, causal, scale, softcap)

@@ -86,19 +86,88 @@ def aligned(x: torch.Tensor) -> torch.Tensor:
 def paged_decode_attention(q: torch.Tensor, kpool: torch.Tensor,
                            vpool: torch.Tensor, block_table: torch.Tensor,
                            lens: torch.Tensor, splits: Optional[int] = None,
-                           scale: Optional[float] = None) -> torch.Tensor:
+                           scale: Optional[float] = None, softcap: float = 0.0,
+                           alibi_slopes: Optional[torch.Tensor] = None
+                           ) -> torch.Tensor:
     """q [n, H, 128] bf16; kpool/vpool [nb, Hkv, BS, 128] bf16;
     block_table [n, max_blocks] int32; lens [n] int32 -> o [n, H, 128].
     The lengths stay on the device, so every request is cut into the same
-    number of splits; ``StepPlan`` cuts by length."""
+    number of splits; ``StepPlan`` cuts by length. With ``softcap`` c the scores
+    are c tanh(score / c), with ``alibi_slopes`` [H] they are less by slope times
+    the distance from the request's last token (its new one): the single-token
+    form of ``masked_attention``. There a block id that is not in the pool gives
+    NaN for its request, and a length of 0 gives 0."""
     ext = get_ext()
     scale = scale if scale is not None else 1.0 / math.sqrt(q.size(-1))
+    if softcap or alibi_slopes is not None:
+        return _shaped(q, kpool, vpool, block_table, lens, splits, scale, softcap,
+                       alibi_slopes)
     if splits is None:
         nw = max(1, q.size(0) * kpool.size(1))
         splits = max(1, min(32, WORKGROUPS // nw))
     return ext.paged_decode(aligned(q), aligned(kpool), aligned(vpool),
                             block_table.contiguous().int(),
                             lens.contiguous().int(), splits, scale)
+
+
+def _shaped(q, kpool, vpool, block_table, lens, splits, scale, softcap, slopes):
+    """``paged_decode_attention`` of capped scores or with a bias by distance."""
+    from .masked_attention import _checked_cap, _checked_slopes
+    what = "paged_decode_attention"
+    softcap = _checked_cap(softcap, what)
+    if q.dim() != 3 or kpool.dim() != 4 or kpool.shape != vpool.shape or \
+            q.shape[2] != kpool.shape[3] or kpool.shape[1] == 0 or \
+            q.shape[1] % kpool.shape[1] or kpool.shape[2] == 0:
+        raise ValueError(f"{what}: q is [n, H, D], the pools are [blocks, Hkv, BS, D] "
+                         f"with H a multiple of Hkv, got {tuple(q.shape)}, "
+                         f"{tuple(kpool.shape)}, {tuple(vpool.shape)}")
+    if block_table.dim() != 2 or block_table.shape[0] != q.shape[0] or \
+            lens.shape != q.shape[:1]:
+        raise ValueError(f"{what}: block_table is [n, blocks], lens [n]")
+    if any(x.device != q.device for x in (kpool, vpool, block_table, lens)):
+        raise ValueError(f"{what}: tensors on different devices")
+    slopes = _checked_slopes(slopes, q, what)
+    ext = get_ext()
+    if not q.is_cuda or ext is None:
+        return _torch_shaped(q, kpool, vpool, block_table, lens, scale, softcap,
+                             slopes)
+    if not paged_decode_available(q, kpool) or kpool.dtype is not torch.bfloat16 or \
+            vpool.dtype is not torch.bfloat16:
+        raise ValueError(f"{what}: bf16, heads of 128 and up to 16 a key head on a GPU")
+    if splits is None:
+        splits = max(1, min(32, WORKGROUPS // max(1, q.size(0) * kpool.size(1))))
+    return ext.paged_decode(aligned(q), aligned(kpool), aligned(vpool),
+                            block_table.contiguous().int(), lens.contiguous().int(),
+                            splits, scale, softcap, slopes)
+
+
+def _torch_shaped(q, kpool, vpool, block_table, lens, scale, softcap, slopes):
+    """The same formulas over the gathered rows, in fp32 (fp64 for fp64)."""
+    n, H, D = q.shape
+    blocks, Hkv, bs, _ = kpool.shape
+    wide = torch.float64 if q.dtype is torch.float64 else torch.float32
+    lens = lens.long().clamp(0, block_table.shape[1] * bs)
+    at = torch.arange(block_table.shape[1] * bs, device=q.device)
+    seen = at < lens[:, None]
+    known = (block_table >= 0) & (block_table < blocks)
+    ids = torch.where(known, block_table, 0).long()
+    # keys past the end are not read: whatever the pool holds there
+    k, v = (pool[ids].to(wide).transpose(2, 3).reshape(n, -1, Hkv, D)
+            .masked_fill(~seen[..., None, None], 0.0).transpose(1, 2)
+            for pool in (kpool, vpool))
+    t = (q.to(wide).view(n, Hkv, H // Hkv, D) @ k.transpose(2, 3).contiguous()) * scale
+    if softcap:
+        t = torch.tanh(t / softcap) * softcap
+    if slopes is not None:
+        t = t - slopes.to(wide).view(Hkv, -1, 1) * \
+            (lens[:, None] - 1 - at)[:, None, None].abs()
+    t = t.masked_fill(~seen[:, None, None], float("-inf"))
+    p = torch.softmax(t, -1)
+    some = (lens > 0)[:, None, None, None]
+    o = torch.where(some, torch.where(seen[:, None, None], p, 0.0) @ v, 0.0)
+    lost = (seen.view(n, -1, bs)[..., 0] & ~known).any(1)
+    o = torch.where(lost[:, None, None, None], float("nan"), o)
+    return o.reshape(n, H, D).to(q.dtype)
 
 
 @dataclass

@@ -1,0 +1,118 @@
+"""Log probabilities of given tokens, with the entropy of their distribution and its
+best tokens (csrc/token_logprobs.hip): what a policy's loss is made of, and what a
+server answers beside its tokens. The logits are read once and nothing of their size is
+written but, backward, their gradient."""
+
+from typing import NamedTuple
+
+import torch
+
+from ._loader import get_ext
+from .linear import untransformed
+
+# Best tokens that a call may ask for, and the vocabulary it may ask them of.
+MOST, WIDEST = 32, 500_000
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprobs`` and ``entropy`` fp32, one a token; ``top_logprobs`` fp32 and
+    ``top_ids`` int64 [.., top], best first, of equal logits the lower id first."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_ids: torch.Tensor
+
+
+def _torch_logprobs(logits, tokens, top, ignore_index):
+    """The formulas in fp32 (fp64 for fp64)."""
+    x = logits if logits.dtype is torch.float64 else logits.float()
+    V = x.shape[-1]
+    live = tokens != ignore_index
+    known = (tokens >= 0) & (tokens < V)
+    x = x.masked_fill(~live[..., None], 0.0)
+    lp = torch.log_softmax(x, -1)
+    # a logit of -inf has no share
+    none = lp == float("-inf")
+    some = lp.masked_fill(none, 0.0)
+    share = torch.where(none, 0.0, some.exp() * some)
+    entropy = torch.where(live, -share.sum(-1), 0.0)
+    got = lp.gather(-1, torch.where(known, tokens, 0)[..., None])[..., 0]
+    got = got * torch.where(known | ~live, 1.0, float("nan")).to(got.dtype)
+    got = torch.where(live, got, 0.0)
+    # NaN above all, as numbers that are equal in order of their ids
+    order = torch.sort(torch.where(x != x, float("inf"), x).detach(), dim=-1,
+                       descending=True, stable=True).indices[..., :top] \
+        if top else tokens.new_empty(*tokens.shape, 0)
+    best = lp.detach().gather(-1, order)
+    return TokenLogprobs(got, entropy,
+                         torch.where(live[..., None], best, float("-inf")),
+                         torch.where(live[..., None], order, -1))
+
+
+def _as_rows(logits):
+    """Logits as the kernels read them: up to three dimensions of any strides but one
+    inside a row."""
+    if logits.dim() > 3:
+        logits = logits.reshape(-1, logits.shape[-2], logits.shape[-1])
+    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    return logits
+
+
+class _LogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, ignore_index):
+        x = _as_rows(logits)
+        lp, entropy, stat, top_lp, top_ids = get_ext().logprobs_fwd(
+            x, tokens, top, ignore_index)
+        ctx.save_for_backward(x, tokens, stat, entropy)
+        ctx.shape, ctx.ignore_index = logits.shape, ignore_index
+        ctx.mark_non_differentiable(top_lp, top_ids)
+        ctx.set_materialize_grads(False)
+        return lp, entropy, top_lp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, glp, gent, _top_lp, _top_ids):
+        if glp is None and gent is None:
+            return None, None, None, None
+        x, tokens, stat, entropy = ctx.saved_tensors
+        glp, gent = (None if g is None else g.float().contiguous()
+                     for g in (glp, gent))
+        dx = get_ext().logprobs_bwd(x, tokens, stat, entropy, glp, gent,
+                                    ctx.ignore_index)
+        return dx.view(ctx.shape), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """``logits`` [.., V] bf16, fp16 or fp32 and ``tokens`` [..] (integers) -> the log
+    probability of each token under the softmax of its logits, the entropy of that
+    softmax in nats, and its ``top`` (up to 32) best tokens with theirs. Differentiable
+    (once) in the logits through ``logprobs`` and ``entropy``. Tokens of
+    ``ignore_index`` give 0 and 0, no gradient, and ids of -1; a token that is not in
+    the vocabulary gives NaN, and a NaN logit counts above all others."""
+    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape or logits.shape[-1] < 1:
+        raise ValueError("token_logprobs: logits [.., V] and tokens [..], got "
+                         f"{tuple(logits.shape)} and {tuple(tokens.shape)}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"token_logprobs: integer tokens, got {tokens.dtype}")
+    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32,
+                            torch.float64):
+        raise ValueError(f"token_logprobs: floating logits, got {logits.dtype}")
+    V = logits.shape[-1]
+    if not 0 <= top <= min(MOST, V) or (top and V > WIDEST):
+        raise ValueError(f"token_logprobs: up to {MOST} best of {WIDEST} tokens at "
+                         f"most, got {top} of {V}")
+    if logits.device != tokens.device:
+        raise ValueError("token_logprobs: tensors on different devices")
+    tokens = tokens.long().contiguous()
+    if not logits.is_cuda or get_ext() is None or not untransformed():
+        return _torch_logprobs(logits, tokens, top, ignore_index)
+    if logits.dtype is torch.float64:
+        raise ValueError("token_logprobs: bf16, fp16 or fp32 on a GPU")
+    lp, entropy, top_lp, top_ids = _LogprobsFn.apply(logits, tokens, top, ignore_index)
+    shape = tokens.shape
+    return TokenLogprobs(lp.view(shape), entropy.view(shape),
+                         top_lp.view(*shape, top), top_ids.view(*shape, top))

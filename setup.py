@@ -50,6 +50,7 @@ ext = CUDAExtension(
     name="deepspeed_amd.ops._C",
     sources=[
         os.path.join(CSRC, "bindings.cpp"),
+        os.path.join(CSRC, "bindings_packed.cpp"),
         os.path.join(CSRC, "cpu_adam.cpp"),
         os.path.join(CSRC, "aio.cpp"),
         os.path.join(CSRC, "shm_comm.cpp"),
@@ -65,6 +66,9 @@ ext = CUDAExtension(
         os.path.join(CSRC, "tile_linear.hip"),
         os.path.join(CSRC, "quantize.hip"),
         os.path.join(CSRC, "attention.hip"),
+        os.path.join(CSRC, "masked_attention.hip"),
+        os.path.join(CSRC, "qk_norm.hip"),
+        os.path.join(CSRC, "token_logprobs.hip"),
         os.path.join(CSRC, "cross_entropy.hip"),
         os.path.join(CSRC, "norms.hip"),
         os.path.join(CSRC, "rope.hip"),

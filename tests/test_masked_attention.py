@@ -1,0 +1,567 @@
+"""Attention over packed rows and its single-token form over the paged pool, against
+the formulas in 64 bits, and what both refuse."""
+
+import math
+
+import pytest
+import torch
+
+from deepspeed_amd.ops.masked_attention import (PackedRows, _torch_spans,
+                                                masked_attention, packed_rows)
+from deepspeed_amd.ops.paged_attention import paged_decode_attention
+
+BF16 = 2.0 ** -8        # a rounding to bf16, relative
+# fp32 scores of up to 128 products and their exponentials, and a tanh of 1 - 2 / (e +
+# 1): less than 2^-14 of a weight for caps and scores up to 100
+FP32 = 2.0 ** -13
+
+
+def _ids(rows, pad=None):
+    """Document ids [B, S] of rows of lengths; negative lengths are padding."""
+    out = []
+    for lens in rows:
+        row, at = [], 0
+        for n in lens:
+            row += [at if n > 0 else -1] * abs(n)
+            at += n > 0
+        out.append(row)
+    return torch.tensor(out, dtype=torch.int32)
+
+
+def _seen(ids, prefix, causal):
+    """[B, S, S] truth values, pair by pair."""
+    B, S = ids.shape
+    seen = torch.zeros(B, S, S, dtype=torch.bool)
+    for b in range(B):
+        row = ids[b].tolist()
+        s = 0
+        while s < S:
+            e = s
+            while e < S and row[e] == row[s]:
+                e += 1
+            if row[s] >= 0:
+                seen[b, s:e, s:e] = True
+                if causal:
+                    seen[b, s:e, s:e] = torch.ones(e - s, e - s).tril().bool()
+                    if prefix is not None and row[s] < prefix.shape[1]:
+                        n = min(e - s, max(0, int(prefix[b, row[s]])))
+                        seen[b, s:e, s:s + n] = True
+            s = e
+    return seen
+
+
+def _reference(q, k, v, do, seen, scale, cap, slopes):
+    """(values, how far off bf16 kernels may be) of o, dq, dk, dv in 64 bits. Hidden
+    pairs are left out of every sum."""
+    B, S, H, D = q.shape
+    Hk = k.shape[2]
+    G = H // Hk
+    q, k, v, do = (x.double().transpose(1, 2) for x in (q, k, v, do))
+    # a hidden row's infinities are nobody's
+    some = seen.any(1)[:, None, :, None]
+    k, v = (torch.where(some, x, 0.0).repeat_interleave(G, 1) for x in (k, v))
+    have = seen.any(2)[:, None, :, None]
+    q, do = (torch.where(have, x, 0.0) for x in (q, do))
+    kt, vt = (x.transpose(2, 3).contiguous() for x in (k, v))
+    seen = seen[:, None]
+    t = (q @ kt) * scale
+    bend = torch.ones_like(t)
+    if cap:
+        bend = 1 - torch.tanh(t / cap) ** 2
+        t = torch.tanh(t / cap) * cap
+    at = torch.arange(S, device=q.device)
+    if slopes is not None:
+        t = t - slopes.double().view(H, 1, 1) * (at[:, None] - at).abs()
+    t = t.masked_fill(~seen, -math.inf)
+    p = torch.where(seen, torch.softmax(t, -1), 0.0)
+    o = p @ v
+    dp = do @ vt
+    delta = (do * o).sum(-1, keepdim=True)
+    ds = torch.where(seen, p * (dp - delta) * bend, 0.0)
+
+    def group(x):
+        return x.view(B, Hk, G, S, D).sum(2)
+
+    pt, dst = p.transpose(2, 3).contiguous(), ds.transpose(2, 3).contiguous()
+    dq, dk, dv = ds @ k * scale, group(dst @ q) * scale, group(pt @ do)
+    # o: weights rounded to bf16, then o itself (kept to 2^-16 for the backward)
+    off_o = (BF16 + FP32) * (p @ v.abs())
+    off_delta = (do.abs() * (off_o + 2.0 ** -15 * o.abs())).sum(-1, keepdim=True)
+    # dS: its own rounding, the sum it is less by, and the weights' fp32
+    off_ds = BF16 * ds.abs() + bend * p * (
+        off_delta + FP32 * (dp.abs() + delta.abs()
+                            + do.abs() @ vt.abs()))
+    off_ds = torch.where(seen, off_ds, 0.0)
+    off = [off_o, off_ds @ k.abs() * abs(scale),
+           group(off_ds.transpose(2, 3).contiguous() @ q.abs()) * abs(scale),
+           group((BF16 + FP32) * (pt @ do.abs()))]
+    values = [x.transpose(1, 2) for x in (o, dq, dk, dv)]
+    # their own rounding; below it bf16's smallest numbers
+    return values, [x.transpose(1, 2) * 1.01 + BF16 * y.abs() + 1e-30
+                    for x, y in zip(off, values)]
+
+
+def _check(got, values, off, names=("o", "dq", "dk", "dv")):
+    for name, x, y, most in zip(names, got, values, off):
+        far = (x.double() - y).abs()
+        assert torch.isfinite(x).all(), name
+        bad = far > most
+        assert not bad.any(), (name, int(bad.sum()), float((far - most).max()),
+                               bad.nonzero()[:4].tolist())
+
+
+def _inputs(B, S, H, Hk, D, device, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, S, H + 2 * Hk, D, generator=g).bfloat16()
+    x[:, :, :H] *= spread
+    do = torch.randn(B, S, H, D, generator=g).bfloat16()
+    x, do = x.to(device), do.to(device)
+    return x[:, :, :H], x[:, :, H:H + Hk], x[:, :, H + Hk:], do
+
+
+def _grads(q, k, v, do, rows, **how):
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    o = masked_attention(q, k, v, rows, **how)
+    return (o.detach(), *torch.autograd.grad(o, (q, k, v), do))
+
+
+DOCUMENTS = [[[1]], [[2], [1, -1]], [[40, 24], [-64]], [[33, 1, 31], [-5, 50, -10]],
+             [[100, 157], [1, 255, -1]], [[64, 64, 128, 65], [321]],
+             [[300, 20, 193], [256, 256, 1]], [[700, -40, 300]]]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("rows", DOCUMENTS)
+def test_spans(rows, causal):
+    """What the spans say is what pair by pair is seen, both ways round, and they
+    grow along a row."""
+    ids = _ids(rows)
+    g = torch.Generator().manual_seed(1)
+    for prefix in [None] + [torch.randint(-2, 90, (len(rows), n), generator=g,
+                                          dtype=torch.int32) for n in (0, 2, 7)]:
+        if prefix is not None and not causal:
+            continue
+        lo, hi, klo, khi = _torch_spans(ids, prefix, causal).long()
+        at = torch.arange(ids.shape[1])
+        seen = _seen(ids, prefix, causal)
+        assert torch.equal((at >= lo[..., None]) & (at < hi[..., None]), seen)
+        assert torch.equal(((at >= klo[..., None]) & (at < khi[..., None]))
+                           .transpose(1, 2), seen)
+        for x in (lo, hi, klo, khi):
+            assert (x[:, 1:] >= x[:, :-1]).all()
+
+
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (2.0, True)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_formulas_cpu(causal, cap, bias):
+    """The plain path on the CPU: values against pair by pair, gradients against
+    differences in 64 bits."""
+    ids = _ids([[5, 3, -2], [1, 6, 3]])
+    prefix = torch.tensor([[2, 9], [0, 3]], dtype=torch.int32) if causal else None
+    rows = packed_rows(ids, prefix, causal)
+    g = torch.Generator().manual_seed(2)
+    q, k, v, do = (torch.randn(2, 10, h, 4, generator=g, dtype=torch.float64)
+                   for h in (4, 2, 2, 4))
+    slopes = torch.tensor([0.5, 0.25, 0.1, 1.0]) if bias else None
+    how = dict(scale=0.7, softcap=cap, alibi_slopes=slopes)
+    values, _ = _reference(q, k, v, do, _seen(ids, prefix, causal), 0.7, cap, slopes)
+    for x, y in zip(_grads(q, k, v, do, rows, **how), values):
+        torch.testing.assert_close(x, y, rtol=1e-9, atol=1e-12)
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    assert torch.autograd.gradcheck(
+        lambda *x: masked_attention(*x, rows, **how), (q, k, v))
+
+
+def test_refusals():
+    q, k, v, _ = _inputs(2, 6, 4, 2, 64, "cpu")
+    ids = _ids([[6], [2, 4]])
+    rows = packed_rows(ids)
+    with pytest.raises(ValueError, match="rows of another batch"):
+        masked_attention(q[:1], k[:1], v[:1], rows)
+    with pytest.raises(ValueError, match="multiple of Hkv"):
+        masked_attention(q[:, :, :3], k, v)
+    with pytest.raises(ValueError, match="multiple of Hkv"):
+        masked_attention(q, k, v[:, :5])
+    with pytest.raises(ValueError, match="one type"):
+        masked_attention(q, k.float(), v.float())
+    for cap in (-1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="softcap"):
+            masked_attention(q, k, v, softcap=cap)
+    with pytest.raises(ValueError, match="one number a query head"):
+        masked_attention(q, k, v, alibi_slopes=torch.ones(2))
+    with pytest.raises(ValueError, match="no gradient"):
+        masked_attention(q, k, v, alibi_slopes=torch.ones(4, requires_grad=True))
+    with pytest.raises(ValueError, match="int32 or int64"):
+        packed_rows(ids.float())
+    with pytest.raises(ValueError, match="without causal"):
+        packed_rows(ids, torch.ones(2, 2, dtype=torch.int32), causal=False)
+    with pytest.raises(ValueError, match="prefix_lens"):
+        packed_rows(ids, torch.ones(3, 2, dtype=torch.int32))
+
+
+def _decode_inputs(lens, H, Hk, bs, device, seed=0, spread=1.0, spare=3):
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // bs) for n in lens]
+    order = torch.randperm(sum(need) + spare, generator=g).int()
+    table = torch.full((len(lens), max(max(need), 1)), -7, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n]
+        at += n
+    pools = [torch.randn(sum(need) + spare, Hk, bs, 128, generator=g).bfloat16()
+             for _ in range(2)]
+    q = torch.randn(len(lens), H, 128, generator=g).bfloat16() * spread
+    return [x.to(device) for x in (q, *pools, table,
+                                   torch.tensor(lens, dtype=torch.int32))]
+
+
+def _decode_reference(q, kpool, vpool, table, lens, scale, cap, slopes):
+    n, H, D = q.shape
+    Hk = kpool.shape[1]
+    out, off = torch.zeros(n, H, D).double(), torch.zeros(n, H, D).double()
+    for i, length in enumerate(lens.tolist()):
+        if not length:
+            continue
+        blocks = table[i, :-(-length // kpool.shape[2])].long()
+        k, v = (x[blocks].double().cpu().transpose(1, 2).reshape(-1, Hk, D)[:length]
+                for x in (kpool, vpool))
+        far = torch.arange(length - 1, -1, -1).double()
+        for h in range(H):
+            t = (k[:, h * Hk // H] @ q[i, h].double().cpu()) * scale
+            if cap:
+                t = torch.tanh(t / cap) * cap
+            if slopes is not None:
+                t = t - float(slopes[h]) * far
+            p = torch.softmax(t, 0)
+            out[i, h] = p @ v[:, h * Hk // H]
+            off[i, h] = FP32 * (p @ v[:, h * Hk // H].abs())
+    return out, off + BF16 * out.abs() + 1e-30
+
+
+@pytest.mark.parametrize("cap,bias", [(0.0, True), (5.0, False), (5.0, True)])
+def test_decode_cpu(cap, bias):
+    """The plain path: as a last row of masked_attention would have it, a bad block
+    NaN for its own request alone, no request 0."""
+    q, kp, vp, table, lens = _decode_inputs([1, 0, 16, 37], 4, 2, 16, "cpu")
+    slopes = torch.tensor([0.5, 0.25, 0.1, 1.0]) if bias else None
+    how = dict(softcap=cap, alibi_slopes=slopes)
+    o = paged_decode_attention(q, kp, vp, table, lens, **how)
+    want, off = _decode_reference(q, kp, vp, table, lens, 128 ** -0.5, cap, slopes)
+    assert ((o.double() - want).abs() <= off).all()
+    assert (o[1] == 0).all()
+    k, v = (x[table[3, :3].long()].transpose(1, 2).reshape(1, -1, 2, 128)[:, :37]
+            for x in (kp, vp))
+    rows = torch.zeros(1, 37, 4, 128).bfloat16()
+    rows[:, -1] = q[3]
+    whole = masked_attention(rows, k, v, **how)[0, -1]
+    torch.testing.assert_close(whole.float(), o[3].float(), rtol=2 * BF16, atol=1e-4)
+    for bad in (-1, kp.shape[0], 2 ** 31 - 1):
+        table[3, 1] = bad
+        again = paged_decode_attention(q, kp, vp, table, lens, **how)
+        assert torch.equal(again[:3], o[:3]) and again[3].isnan().all()
+
+
+def test_decode_refusals():
+    q, kp, vp, table, lens = _decode_inputs([5, 9], 4, 2, 16, "cpu")
+    with pytest.raises(ValueError, match="softcap"):
+        paged_decode_attention(q, kp, vp, table, lens, softcap=-1.0)
+    with pytest.raises(ValueError, match="one number a query head"):
+        paged_decode_attention(q, kp, vp, table, lens, alibi_slopes=torch.ones(3))
+    with pytest.raises(ValueError, match="multiple of Hkv"):
+        paged_decode_attention(q[:, :3], kp, vp, table, lens, softcap=1.0)
+    with pytest.raises(ValueError, match="block_table"):
+        paged_decode_attention(q, kp, vp, table[:1], lens, softcap=1.0)
+
+
+# ------------------------------------------------------------------------- GPU
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("rows", DOCUMENTS + [[[5000, 1, 7000, 3000]], [[20000]],
+                                              [[4095, 4097, -1], [1, 8191, 1]],
+                                              [[1] * 1500]])
+def test_spans_gpu(rows, causal):
+    ids = _ids(rows)
+    g = torch.Generator().manual_seed(1)
+    for prefix in [None] + [torch.randint(-2, 90, (len(rows), n), generator=g,
+                                          dtype=torch.int32) for n in (0, 2, 7)]:
+        if prefix is not None and not causal:
+            continue
+        want = _torch_spans(ids, prefix, causal)
+        for kind in (torch.int32, torch.int64):
+            got = packed_rows(ids.to("cuda", kind),
+                              None if prefix is None else prefix.to("cuda", kind),
+                              causal)
+            assert got.spans.dtype is torch.int32
+            assert torch.equal(got.spans.cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap,bias,spread", [(0.0, False, 1), (0.0, True, 1),
+                                             (20.0, False, 4), (5.0, True, 2)])
+@pytest.mark.parametrize("heads", [(2, 2, 64), (4, 2, 96), (6, 1, 128), (8, 8, 64)])
+@pytest.mark.parametrize("rows", DOCUMENTS)
+def test_documents_gpu(rows, heads, cap, bias, spread):
+    H, Hk, D = heads
+    ids = _ids(rows)
+    B, S = ids.shape
+    q, k, v, do = _inputs(B, S, H, Hk, D, "cuda", spread=spread)
+    slopes = torch.exp2(-torch.arange(1, H + 1).float()).cuda() if bias else None
+    g = torch.Generator().manual_seed(3)
+    prefix = torch.randint(0, 60, (B, 3), generator=g, dtype=torch.int32)
+    for causal, pre in ((True, None), (True, prefix), (False, None)):
+        packed = packed_rows(ids.cuda(), None if pre is None else pre.cuda(), causal)
+        got = _grads(q, k, v, do, packed, softcap=cap, alibi_slopes=slopes)
+        seen = _seen(ids, pre, causal).cuda()
+        _check(got, *_reference(q, k, v, do, seen, D ** -0.5, cap, slopes))
+        empty = ~seen.any(2)
+        for x in got[:2]:
+            assert (x[empty] == 0).all()
+        for x in got[2:]:
+            assert (x[~seen.any(1)] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("S", [1, 3, 64, 129, 511])
+@pytest.mark.parametrize("scale", [None, -0.2, 0.0])
+def test_without_rows_gpu(S, causal, scale):
+    q, k, v, do = _inputs(2, S, 4, 2, 128, "cuda", seed=S)
+    at = torch.arange(S)
+    seen = (at <= at[:, None] if causal else at == at).expand(2, S, S).cuda()
+    slopes = torch.tensor([0.5, 0.1, 0.0, 2.0]).cuda()
+    for cap, sl in ((0.0, None), (10.0, None), (3.0, slopes)):
+        got = _grads(q, k, v, do, None, causal=causal, scale=scale, softcap=cap,
+                     alibi_slopes=sl)
+        _check(got, *_reference(q, k, v, do, seen,
+                                128 ** -0.5 if scale is None else scale, cap, sl))
+
+
+@pytest.mark.gpu
+def test_long_rows_gpu():
+    """Splits of the gradients of shared heads, many tiles, uneven documents."""
+    ids = _ids([[1500, 30, 2, 400, 1068, -96]])
+    q, k, v, do = _inputs(1, ids.shape[1], 8, 2, 128, "cuda", seed=5, spread=3)
+    prefix = torch.tensor([[700, 30, 5, 0, 1]], dtype=torch.int32)
+    rows = packed_rows(ids.cuda(), prefix.cuda())
+    got = _grads(q, k, v, do, rows, softcap=30.0)
+    seen = _seen(ids, prefix, True).cuda()
+    _check(got, *_reference(q, k, v, do, seen, 128 ** -0.5, 30.0, None))
+    again = _grads(q, k, v, do, rows, softcap=30.0)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (10.0, True)])
+def test_hidden_infinities_gpu(value, cap, bias):
+    """What a query does not see is not in its row, whatever it holds: padding,
+    another document, a later token."""
+    ids = _ids([[70, 60, -30], [-3, 50, 107]])
+    H, Hk, D = 4, 2, 64
+    slopes = torch.tensor([0.5, 0.1, 0.0, 2.0]).cuda() if bias else None
+    how = dict(softcap=cap, alibi_slopes=slopes)
+    rows = packed_rows(ids.cuda())
+    seen = _seen(ids, None, True).cuda()
+    q, k, v, do = _inputs(2, 160, H, Hk, D, "cuda", seed=7)
+    pad = (ids < 0).cuda()
+    for x in (q, k, v, do):
+        x[pad] = value
+    got = _grads(q, k, v, do, rows, **how)
+    want = _reference(q, k, v, do, seen, D ** -0.5, cap, slopes)
+    _check(got, *want)
+    for x in (got[0], got[1], got[2], got[3]):
+        assert (x[pad] == 0).all()
+    # one key and value of the first document, seen by its last 5 tokens only
+    sick_k, sick_v = k.clone(), v.clone()
+    sick_v[0, 65] = value
+    o = masked_attention(q, sick_k, sick_v, rows, **how)
+    well = torch.ones(2, 160, dtype=torch.bool)
+    well[0, 65:70] = False
+    assert torch.equal(torch.isfinite(o).all(-1).all(-1).cpu(), well)
+    far = (o.double() - want[0][0]).abs() <= want[1][0]
+    assert far[well].all()
+    # and its gradients: rows of the other documents are as they were
+    got = _grads(q, sick_k, sick_v, do, rows, **how)
+    other = (ids != ids[0, 0]).cuda()
+    other[1] = True
+    for x, y, off in zip(got[1:], want[0][1:], want[1][1:]):
+        assert ((x.double() - y).abs() <= off)[other].all()
+
+
+@pytest.mark.gpu
+def test_layouts_gpu():
+    """Strides, alignment and broadcast inputs other than a joint projection's."""
+    ids = _ids([[90, 40], [20, 110]])
+    rows = packed_rows(ids.cuda())
+    seen = _seen(ids, None, True).cuda()
+    q, k, v, do = _inputs(2, 130, 4, 2, 64, "cuda", seed=9)
+    want = _reference(q, k, v, do, seen, 0.125, 0.0, None)
+
+    def heads_first(x):
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+
+    def odd(x):
+        flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+        flat[1:] = x.reshape(-1)
+        return flat[1:].view(x.shape)
+
+    def spread(x):
+        wide = torch.empty(*x.shape[:3], 2 * x.shape[3], dtype=x.dtype, device=x.device)
+        wide[..., ::2] = x
+        return wide[..., ::2]
+
+    for change in (heads_first, odd, spread):
+        _check(_grads(*(change(x) for x in (q, k, v, do)), rows), *want)
+    # one batch row's key for both rows; an expanded gradient
+    k1 = k[:1].expand(2, -1, -1, -1)
+    one = do[:, :1, :1].expand(2, 130, 4, 64)
+    want = _reference(q, k1, v, one, seen, 0.125, 0.0, None)
+    _check(_grads(q, k1, v, one, rows), *want)
+    leaf = k[:1].detach().requires_grad_()
+    o = masked_attention(q, leaf.expand(2, -1, -1, -1), v, rows)
+    dk, = torch.autograd.grad(o, leaf, one)
+    # of a sum in bf16 of two rows: each term's and the sum's rounding
+    y, off = want[0][2], want[1][2]
+    assert ((dk.double() - y.sum(0)).abs() <= off.sum(0) + 2 * BF16 * y.abs().sum(0)
+            ).all()
+
+
+@pytest.mark.gpu
+def test_differences_gpu():
+    """The kernels' gradients against differences of the formulas in 64 bits."""
+    ids = _ids([[100, 41]])
+    prefix = torch.tensor([[30, 0]], dtype=torch.int32)
+    seen = _seen(ids, prefix, True).cuda()
+    slopes = torch.tensor([0.3, 0.05]).cuda()
+    q, k, v, do = _inputs(1, 141, 2, 1, 96, "cuda", seed=11, spread=2)
+    rows = packed_rows(ids.cuda(), prefix.cuda())
+    got = _grads(q, k, v, do, rows, softcap=8.0, alibi_slopes=slopes)
+
+    def loss(*x):
+        o = _reference(*x, do, seen, 96 ** -0.5, 8.0, slopes)[0][0]
+        return float((o * do.double()).sum())
+
+    _, off = _reference(q, k, v, do, seen, 96 ** -0.5, 8.0, slopes)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for i in range(3):
+        x = [t.double() for t in (q, k, v)]
+        u = torch.randn(x[i].shape, generator=g, device="cuda", dtype=torch.float64)
+        ends = []
+        for step in (1e-5, -1e-5):
+            y = list(x)
+            y[i] = x[i] + step * u
+            ends.append(loss(*y))
+        slope = (ends[0] - ends[1]) / 2e-5
+        most = float((off[i + 1] * u.abs()).sum()) + 1e-4
+        assert abs(slope - float((got[i + 1].double() * u).sum())) <= most
+
+
+@pytest.mark.gpu
+def test_graph_and_streams_gpu():
+    """Captured with its backward and replayed over changing inputs beside eager
+    calls; and on another stream than the current one's."""
+    ids = _ids([[150, 90], [60, 160, -20]]).cuda()
+    static = [x.clone() for x in _inputs(2, 240, 4, 2, 64, "cuda")]
+
+    def step(q, k, v, do):
+        return _grads(q, k, v, do, packed_rows(ids), softcap=10.0)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for seed in range(4):
+        fresh = _inputs(2, 240, 4, 2, 64, "cuda", seed=20 + seed)
+        want = step(*fresh)
+        for x, y in zip(static, fresh):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            there = step(*fresh)
+        side.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(there, want))
+
+
+@pytest.mark.gpu
+def test_refusals_gpu():
+    q, k, v, _ = _inputs(1, 8, 2, 2, 64, "cuda")
+    with pytest.raises(ValueError, match="bf16"):
+        masked_attention(q.half(), k.half(), v.half())
+    with pytest.raises(ValueError, match="heads of 64"):
+        masked_attention(q[..., :32], k[..., :32], v[..., :32])
+    with pytest.raises(ValueError, match="device"):
+        masked_attention(q, k, v, packed_rows(torch.zeros(1, 8, dtype=torch.int32)))
+    empty = torch.empty(0, 8, 2, 64, dtype=torch.bfloat16, device="cuda")
+    assert masked_attention(empty, empty, empty).shape == empty.shape
+    none = torch.empty(2, 0, 2, 64, dtype=torch.bfloat16, device="cuda",
+                       requires_grad=True)
+    ids = torch.empty(2, 0, dtype=torch.int32, device="cuda")
+    masked_attention(none, none, none, packed_rows(ids)).sum().backward()
+    # spans that say more than there is read nothing outside of the rows
+    wild = torch.full((4, 1, 8), 2 ** 31 - 1, dtype=torch.int32, device="cuda")
+    wild[::2] = -2 ** 31
+    full = masked_attention(q, k, v, causal=False)
+    assert torch.equal(masked_attention(q, k, v, PackedRows(wild, False)), full)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap,bias,spread", [(0.0, True, 1), (30.0, False, 4),
+                                             (5.0, True, 2)])
+@pytest.mark.parametrize("lens,heads,bs", [
+    ([1], (8, 8), 64), ([33, 0, 1, 64], (32, 8), 64), ([31, 32, 500], (28, 4), 16),
+    ([130, 129], (16, 1), 32), ([7, 300], (5, 5), 5), ([3000, 10, 700], (32, 8), 128)])
+@pytest.mark.parametrize("splits", [None, 1, 7])
+def test_decode_gpu(lens, heads, bs, splits, cap, bias, spread):
+    H, Hk = heads
+    q, kp, vp, table, n = _decode_inputs(lens, H, Hk, bs, "cuda", spread=spread)
+    slopes = torch.exp2(-torch.arange(1, H + 1).float() / 4).cuda() if bias else None
+    for scale in (None, -0.1):
+        o = paged_decode_attention(q, kp, vp, table, n, splits=splits, scale=scale,
+                                   softcap=cap, alibi_slopes=slopes)
+        want, off = _decode_reference(q, kp, vp, table, n,
+                                      128 ** -0.5 if scale is None else scale, cap,
+                                      slopes)
+        assert ((o.double().cpu() - want).abs() <= off).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [16, 64])
+def test_decode_bad_pages_gpu(bs):
+    """A block that is not in the pool, and a length past the table's end."""
+    q, kp, vp, table, n = _decode_inputs([100, 200, 40], 8, 2, bs, "cuda")
+    slopes = torch.full((8,), 0.1).cuda()
+    o = paged_decode_attention(q, kp, vp, table, n, softcap=10.0, alibi_slopes=slopes)
+    for bad in (-1, kp.shape[0], 2 ** 31 - 1, -2 ** 31):
+        sick = table.clone()
+        sick[1, 2] = bad
+        for splits in (None, 1, 3):
+            got = paged_decode_attention(q, kp, vp, sick, n, splits=splits,
+                                         softcap=10.0, alibi_slopes=slopes)
+            assert got[1].isnan().all() and torch.isfinite(got[[0, 2]]).all()
+    # what lies behind a request's last key does not count
+    vp2, kp2 = vp.clone(), kp.clone()
+    last = int(table[0, 100 // bs])
+    kp2[last, :, 100 % bs:] = float("nan")
+    vp2[last, :, 100 % bs:] = float("nan")
+    again = paged_decode_attention(q, kp2, vp2, table, n, softcap=10.0,
+                                   alibi_slopes=slopes)
+    assert torch.equal(again, o)
+    long = n.clone()
+    long[1] = 2 ** 31 - 1
+    table[1] = table[1].clamp(min=0)
+    most = n.clone()
+    most[1] = table.shape[1] * bs
+    assert torch.equal(paged_decode_attention(q, kp, vp, table, long, softcap=10.0),
+                       paged_decode_attention(q, kp, vp, table, most, softcap=10.0))
+    with pytest.raises(ValueError, match="up to 16 a key head"):
+        paged_decode_attention(q.float(), kp, vp, table, n, softcap=1.0)
