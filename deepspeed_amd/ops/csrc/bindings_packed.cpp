@@ -80,8 +80,8 @@ struct MaskedArgs : FlashArgs {
              const Opt& spans_, const Opt& slopes_, double scale, double cap)
       : FlashArgs(q, k, v, scale) {
     TORCH_CHECK(cap >= 0 && cap < 1e30, "masked_attention: softcap");
-    TORCH_CHECK((int64_t)B * H * ((S + 127) / 128) * 256 < THREADS &&
-                (int64_t)B * S * H * 16 < THREADS, "masked_attention: size");
+    TORCH_CHECK((int64_t)B * H * ((S + 127) / 128) * 256 < THREADS,
+                "masked_attention: size");
     if (data(spans_)) {
       TORCH_CHECK(spans_->scalar_type() == at::kInt &&
                   spans_->is_contiguous() && spans_->dim() == 3 &&
@@ -134,7 +134,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_bwd(
   auto dq = at::empty({a.B, a.S, a.H, a.D}, q.options());
   auto dk = at::empty({a.B, a.S, a.Hkv, a.D}, q.options());
   auto dv = at::empty({a.B, a.S, a.Hkv, a.D}, q.options());
-  auto stat = at::empty({2, lse.numel()}, lse.options());
+  auto stat = at::empty_like(lse);
   auto part = at::empty({splits > 1 ? 2 * splits * dk.numel() : 0},
                         lse.options());
   a.add(q, q); a.add(k, k); a.add(v, k); a.add(o, q); a.add(dout, q);

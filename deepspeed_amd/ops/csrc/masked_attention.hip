@@ -28,7 +28,6 @@ namespace {
 using namespace attn;
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 struct View {             // element strides of [B, S, H, D]
@@ -38,9 +37,9 @@ struct View {             // element strides of [B, S, H, D]
 struct Args {
   const short *q, *k, *v, *o, *dout;
   short *out, *dq, *dk, *dv;
-  float* lse;
+  float* lse;             // in units of log2
   int* rest;              // [B, S, H, D] bytes: what `out` was rounded by, or null
-  float* stat;            // [2][B, H, S]: lse log2(e), sum(do * o)
+  float* stat;            // [B, H, S]: sum(do * o), from dQ's pass to dK's
   float* part;            // splits of dK and dV, or null
   const int* spans;       // [4][B, S]: q lo, q hi, k lo, k hi, or null
   const float* slopes;    // [H]
@@ -83,22 +82,36 @@ __device__ __forceinline__ bool finite(float x) {
   return __builtin_fabsf(x) < __builtin_inff();
 }
 
+// t and the eight numbers of an operand.
+__device__ __forceinline__ float add_pairs(s16x8 x, float t) {
+  const b16x8 y = __builtin_bit_cast(b16x8, x);
+  const b16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    t = __builtin_amdgcn_fdot2_f32_bf16(b16x2{y[2 * i], y[2 * i + 1]}, one, t,
+                                        false);
+  return t;
+}
+
 // Scores in units of log2, with their derivative's factor where that is asked for.
-// tanh x = 1 - 2 / (e^2x + 1) holds for every x, infinities among them.
+// tanh x = 1 - 2 / (e^2x + 1) holds for every x, infinities among them. (A polynomial
+// where all of a tile's scores are near 0 takes two thirds of its instructions and was
+// 4% less of the forward and nothing of the rest: the matrix cores' operands, not
+// these, are what a step waits for.)
 template <bool CAP, bool BIAS>
 struct Score {
-  static constexpr bool PLAIN = !CAP && !BIAS;
-  float c, a, cap, slope;
+  const Args& a;
+  const float slope;
   __device__ __forceinline__ float operator()(float s, float far,
                                               float& bend) const {
     float t;
     if (CAP) {
       const float r =
-          __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a) + 1.f);
-      t = __builtin_fmaf(-2.f * cap, r, cap);
+          __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.a) + 1.f);
+      t = __builtin_fmaf(-2.f * a.cap, r, a.cap);
       bend = 4.f * r * (1.f - r);
     } else {
-      t = s * c;
+      t = s * a.c;
     }
     if (BIAS) t = __builtin_fmaf(-__builtin_fabsf(far), slope, t);
     return t;
@@ -142,13 +155,22 @@ __device__ __forceinline__ unsigned rests(float a, float b, int ab, float c,
          rest_of(c, cd << 16) << 16 | rest_of(d, cd & 0xffff0000) << 24;
 }
 
+// Loads into registers end here, before a loop: the compiler, which does not know of the
+// tiles' loads, would wait for these where it first uses them, in every step of the
+// loop, and so for the next tile's as well.
+template <int N>
+__device__ __forceinline__ void settle(s16x8 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(x[i]));
+}
+
 // ------------------------------------------------------------------ forward
 
-template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(512) void fwd_kernel(const Args a,
-                                                  const int blocks,
-                                                  const int heads) {
-  constexpr int KB = 64, DB = D / 32, KK = D / 16;
+template <int D, bool CAP, bool BIAS, int NW, int KB>
+__global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(const Args a,
+                                                         const int blocks,
+                                                         const int heads) {
+  constexpr int KT = KB / 32, DB = D / 32, KK = D / 16, QB = 32 * NW, TPB = 64 * NW;
   constexpr bool PLAIN = !CAP && !BIAS;
   using T = Tile<D>;
   __shared__ __attribute__((aligned(16))) short kt[2][KB * T::SC * 8];
@@ -162,19 +184,13 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
   place(blockIdx.x, blocks, heads, blk, bh);
   blk = blocks - 1 - blk;
   const int b = bh / a.H, h = bh % a.H, hkv = h / (a.H / a.Hkv);
-  const int q0b = blk * 256, q0 = q0b + wid * 32, row = q0 + col;
+  const int q0b = blk * QB, q0 = q0b + wid * 32, row = q0 + col;
   const int at = min(row, S - 1);
 
   const short* kp = a.k + b * a.vk.b + hkv * a.vk.h;
   const short* vp = a.v + b * a.vv.b + hkv * a.vv.h;
   const short* qp = a.q + b * a.vq.b + h * a.vq.h + at * a.vq.s;
-  s16x8 qf[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk)
-    qf[kk] = *(const s16x8*)(qp + 16 * kk + 8 * half);
-
-  const Score<CAP, BIAS> score = {a.c, a.a, a.cap,
-                                  BIAS ? a.slopes[h] * LOG2E : 0.f};
+  const Score<CAP, BIAS> score = {a, BIAS ? a.slopes[h] * LOG2E : 0.f};
   const float c = PLAIN ? a.c : 1.f;
   const Span me = span(a, b, at, false);
   const int width = max(me.hi - me.lo, 0);
@@ -183,29 +199,35 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
   const int all1 = lane_of(me.hi, 0);
   const int any1 = q0 < S ? lane_of(me.hi, 31) : 0;
   const int k_begin = uni(span(a, b, q0b, false).lo);
-  const int k_end = uni(span(a, b, min(q0b + 255, S - 1), false).hi);
+  const int k_end = uni(span(a, b, min(q0b + QB - 1, S - 1), false).hi);
   const int steps = (k_end - k_begin + KB - 1) / KB;
 
-  float m = -1e30f, l = 0.f;
+  // sums of the weights, and of the weights as they are rounded for the product: o is
+  // over these, so that the rounding of a weight that is most of its row goes out
+  float m = -1e30f, l = 0.f, lr = 0.f;
   f32x16 acc[DB] = {};
   auto fetch = [&](int k0, int buf) __attribute__((always_inline)) {
-    T::template fetch<KB, 512>(kp + k0 * a.vk.s, (int)a.vk.s, S - k0, kt[buf],
+    T::template fetch<KB, TPB>(kp + k0 * a.vk.s, (int)a.vk.s, S - k0, kt[buf],
                                tid);
-    T::template fetch<KB, 512>(vp + k0 * a.vv.s, (int)a.vv.s, S - k0, vt[buf],
+    T::template fetch<KB, TPB>(vp + k0 * a.vv.s, (int)a.vv.s, S - k0, vt[buf],
                                tid);
   };
-  if (steps > 0) {
-    fetch(k_begin, 0);
-    arrive();
-  }
+  // the queries behind the first tile: one wait for both
+  if (steps > 0) fetch(k_begin, 0);
+  s16x8 qf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk)
+    qf[kk] = *(const s16x8*)(qp + 16 * kk + 8 * half);
+  arrive();
+  settle(qf);
   for (int it = 0; it < steps; ++it) {
     const int k0 = k_begin + it * KB, cur = it & 1;
     if (it + 1 < steps) fetch(k0 + KB, cur ^ 1);
     if (k0 < any1 && k0 + KB > any0) {
-      f32x16 p[2] = {};
+      f32x16 p[KT] = {};
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
           p[t] = mfma(T::rows(kt[cur], 32 * t, kk, ra), qf[kk], p[t]);
@@ -213,18 +235,18 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
       if (!PLAIN) {
         const float far = (float)(k0 + 4 * half - at);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             float bend;
-            p[t][r] = score(p[t][r], far + (32 * t + (r & 3) + 8 * (r >> 2)),
-                            bend);
+            p[t][r] = score(
+                p[t][r], far + (32 * t + (r & 3) + 8 * (r >> 2)), bend);
           }
       }
       if (k0 < all0 || k0 + KB > all1) {
         const int first = me.lo - k0 - 4 * half;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if ((unsigned)(32 * t + (r & 3) + 8 * (r >> 2) - first) >=
@@ -233,7 +255,7 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
       }
       float mt = -1e30f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, p[t][r]);
       mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
@@ -242,6 +264,7 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
         const float alpha = __builtin_amdgcn_exp2f((m - mn) * c);
         m = mn;
         l *= alpha;
+        lr *= alpha;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -250,7 +273,7 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
       const float mc = m * c;
       float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
           const float x0 = PLAIN ? __builtin_fmaf(p[t][r], c, -mc)
@@ -265,10 +288,11 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
       l += l0 + l1;
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const s16x8 pb = operand(p[t], s);
+          lr = add_pairs(pb, lr);
 #pragma unroll
           for (int db = 0; db < DB; ++db)
             acc[db] =
@@ -280,8 +304,9 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
   }
 
   l += __shfl_xor(l, 32, 64);
+  lr += __shfl_xor(lr, 32, 64);
   // a row that sees nothing is 0, and its logarithm of nothing -inf
-  const float inv = width == 0 ? 0.f : 1.f / l;
+  const float inv = width == 0 ? 0.f : 1.f / lr;
   bool good = true;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -294,7 +319,7 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
   const float sum = m * c + __builtin_amdgcn_logf(l);      // log2
   if (real && half == 0)
     a.lse[((long long)b * a.H + h) * S + row] =
-        width == 0 ? -__builtin_inff() : sum * LN2;
+        width == 0 ? -__builtin_inff() : sum;
   short* const op = a.out + b * a.vo.b + h * a.vo.h;
   if (real) {
     short* y = op + row * a.vo.s + 4 * half;
@@ -345,45 +370,11 @@ __global__ __launch_bounds__(512) void fwd_kernel(const Args a,
 
 // ----------------------------------------------------------------- backward
 
-template <int D>
-__global__ __launch_bounds__(256) void stat_kernel(const Args a,
-                                                   const long long rows) {
-  const int sub = threadIdx.x & 15;
-  const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (u >= rows) return;               // u = (b S + s) H + h
-  const int h = (int)(u % a.H);
-  const long long bs = u / a.H;
-  const int s = (int)(bs % a.S);
-  const long long b = bs / a.S;
-  float sum = 0.f;
-  if (8 * sub < D) {
-    const s16x8 x = *(const s16x8*)(a.dout + b * a.vd.b + s * a.vd.s +
-                                    h * a.vd.h + 8 * sub);
-    const s16x8 y = *(const s16x8*)(a.o + b * a.vo.b + s * a.vo.s +
-                                    h * a.vo.h + 8 * sub);
-    const i32x2 r = *(const i32x2*)(a.rest + (u * D + 8 * sub) / 4);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int more = (r[e >> 2] << (24 - 8 * (e & 3))) >> 24;   // signed
-      const int o = ((int)(unsigned short)y[e] << 16) + more * 256;
-      sum += value(x[e]) * __builtin_bit_cast(float, o);
-    }
-  }
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if (sub == 0) {
-    const long long at = (b * a.H + h) * a.S + s;
-    a.stat[at] = a.lse[at] * LOG2E;
-    a.stat[rows + at] = sum;
-  }
-}
-
 // dK and dV: a wave owns 32 keys and walks the queries that see them.
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
                                                       const int blocks,
-                                                      const int heads,
-                                                      const long long rows) {
+                                                      const int heads) {
   constexpr int QB = 64, DB = D / 32, KK = D / 16;
   constexpr bool PLAIN = !CAP && !BIAS;
   using T = Tile<D>;
@@ -401,14 +392,6 @@ __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
   const int k0b = blk * 128, k0 = k0b + wid * 32, key = k0 + col;
   const int at = min(key, S - 1);
 
-  const short* kp = a.k + b * a.vk.b + hkv * a.vk.h + at * a.vk.s;
-  const short* vp = a.v + b * a.vv.b + hkv * a.vv.h + at * a.vv.s;
-  s16x8 kf[KK], vf[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) {
-    kf[kk] = *(const s16x8*)(kp + 16 * kk + 8 * half);
-    vf[kk] = *(const s16x8*)(vp + 16 * kk + 8 * half);
-  }
   f32x16 dka[DB] = {}, dva[DB] = {};
 
   const Span me = span(a, b, at, true);
@@ -430,21 +413,28 @@ __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
     T::template fetch<QB, 256>(a.dout + b * a.vd.b + h * a.vd.h + s0 * a.vd.s,
                                (int)a.vd.s, S - s0, dt[buf], tid);
     if (wid < 2) {
-      const float* p =
-          a.stat + wid * rows + ((long long)b * a.H + h) * S + s0;
+      const float* p = (wid ? a.stat : a.lse) +
+                       ((long long)b * a.H + h) * S + s0;
       load_lds<4>(p, 4u * min(lane, S - s0 - 1), lds_at(&st[buf][wid][0]));
     }
   };
 
   int h = hkv * G + g0, s0 = first;
-  if (steps > 0) {
-    fetch(h, s0, 0, tid);
-    arrive();
+  if (steps > 0) fetch(h, s0, 0, tid);
+  const short* kp = a.k + b * a.vk.b + hkv * a.vk.h + at * a.vk.s;
+  const short* vp = a.v + b * a.vv.b + hkv * a.vv.h + at * a.vv.s;
+  s16x8 kf[KK], vf[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    kf[kk] = *(const s16x8*)(kp + 16 * kk + 8 * half);
+    vf[kk] = *(const s16x8*)(vp + 16 * kk + 8 * half);
   }
+  arrive();
+  settle(kf);
+  settle(vf);
   for (int it = 0; it < steps; ++it) {
     const int cur = it & 1;
-    const Score<CAP, BIAS> score = {a.c, a.a, a.cap,
-                                    BIAS ? a.slopes[h] * LOG2E : 0.f};
+    const Score<CAP, BIAS> score = {a, BIAS ? a.slopes[h] * LOG2E : 0.f};
     int s1 = s0 + QB;
     if (s1 >= last) {
       s1 = first;
@@ -473,15 +463,17 @@ __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
       const float far = (float)(r0 + 4 * half - at);
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 ls = *(const f32x4*)&st[cur][0][32 * t + 8 * g + 4 * half];
-        const f32x4 dl = *(const f32x4*)&st[cur][1][32 * t + 8 * g + 4 * half];
+        const int i = 32 * t + 8 * g + 4 * half;
+        const f32x4 ls = *(const f32x4*)&st[cur][0][i];
+        const f32x4 dl = *(const f32x4*)&st[cur][1][i];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
           float bend = 1.f;
-          const float x =
-              PLAIN ? __builtin_fmaf(p[r], a.c, -ls[e])
-                    : score(p[r], far + (8 * g + e), bend) - ls[e];
+          const float x = PLAIN
+                              ? __builtin_fmaf(p[r], a.c, -ls[e])
+                              : score(
+                                    p[r], far + (8 * g + e), bend) - ls[e];
           p[r] = __builtin_amdgcn_exp2f(x);
           dp[r] -= dl[e];
           if (CAP) dp[r] *= bend;
@@ -565,16 +557,16 @@ __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
     const short* vj = a.v + b * a.vv.b + hkv * a.vv.h + j * a.vv.s;
     float k_0 = 0.f, k_1 = 0.f, v_0 = 0.f, v_1 = 0.f;
     for (int head = hkv * G + g0; head < hkv * G + g1; ++head) {
-      const Score<CAP, BIAS> score = {a.c, a.a, a.cap,
-                                      BIAS ? a.slopes[head] * LOG2E : 0.f};
-      const float* ls = a.stat + ((long long)b * a.H + head) * S;
+      const Score<CAP, BIAS> score = {a, BIAS ? a.slopes[head] * LOG2E : 0.f};
+      const float* ls = a.lse + ((long long)b * a.H + head) * S;
+      const float* dl = a.stat + ((long long)b * a.H + head) * S;
       for (int i = lo; i < hi; ++i) {
         const short* qi = a.q + b * a.vq.b + head * a.vq.h + i * a.vq.s;
         const short* di = a.dout + b * a.vd.b + head * a.vd.h + i * a.vd.s;
         float bend = 1.f;
         const float t = score(dot<D>(qi, kj, lane), (float)(i - j), bend);
         const float p = __builtin_amdgcn_exp2f(t - ls[i]);
-        float ds = (dot<D>(di, vj, lane) - ls[rows + i]) * p;
+        float ds = (dot<D>(di, vj, lane) - dl[i]) * p;
         if (CAP) ds *= bend;
         if (lane < D) {
           k_0 += ds * value(qi[lane]);
@@ -630,8 +622,7 @@ __global__ __launch_bounds__(256) void add_kernel(
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
                                                     const int blocks,
-                                                    const int heads,
-                                                    const long long rows) {
+                                                    const int heads) {
   constexpr int KB = 64, DB = D / 32, KK = D / 16;
   constexpr bool PLAIN = !CAP && !BIAS;
   using T = Tile<D>;
@@ -653,18 +644,9 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
   const short* qb = a.q + b * a.vq.b + h * a.vq.h;
   const short* db_ = a.dout + b * a.vd.b + h * a.vd.h;
 
-  s16x8 qf[KK], df[KK];
-#pragma unroll
-  for (int kk = 0; kk < KK; ++kk) {
-    qf[kk] = *(const s16x8*)(qb + at * a.vq.s + 16 * kk + 8 * half);
-    df[kk] = *(const s16x8*)(db_ + at * a.vd.s + 16 * kk + 8 * half);
-  }
-  const long long sat = ((long long)b * a.H + h) * S + at;
-  const float ls = a.stat[sat], dl = a.stat[rows + sat];
   f32x16 acc[DB] = {};
 
-  const Score<CAP, BIAS> score = {a.c, a.a, a.cap,
-                                  BIAS ? a.slopes[h] * LOG2E : 0.f};
+  const Score<CAP, BIAS> score = {a, BIAS ? a.slopes[h] * LOG2E : 0.f};
   const Span me = span(a, b, at, false);
   const int width = max(me.hi - me.lo, 0);
   const int any0 = lane_of(me.lo, 0), all0 = lane_of(me.lo, 31);
@@ -680,10 +662,37 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
     T::template fetch<KB, 256>(vp + k0 * a.vv.s, (int)a.vv.s, S - k0, vt[buf],
                                tid);
   };
-  if (steps > 0) {
-    fetch(k_begin, 0);
-    arrive();
+  // the rows behind the first tile: one wait for all
+  if (steps > 0) fetch(k_begin, 0);
+  s16x8 qf[KK], df[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    qf[kk] = *(const s16x8*)(qb + at * a.vq.s + 16 * kk + 8 * half);
+    df[kk] = *(const s16x8*)(db_ + at * a.vd.s + 16 * kk + 8 * half);
   }
+  const long long sat = ((long long)b * a.H + h) * S + at;
+  const float ls = a.lse[sat];
+  float dl = 0.f;
+  {
+    const short* op = a.o + b * a.vo.b + h * a.vo.h + at * a.vo.s;
+    const int* rp = a.rest + (((long long)b * S + at) * a.H + h) * (D / 4);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const s16x8 y = *(const s16x8*)(op + 16 * kk + 8 * half);
+      const i32x2 r = *(const i32x2*)(rp + 4 * kk + 2 * half);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int more = (r[e >> 2] << (24 - 8 * (e & 3))) >> 24;   // signed
+        const int o = ((int)(unsigned short)y[e] << 16) + more * 256;
+        dl = __builtin_fmaf(value(df[kk][e]), __builtin_bit_cast(float, o), dl);
+      }
+    }
+    dl += __shfl_xor(dl, 32, 64);
+    if (row < S && half == 0) a.stat[sat] = dl;
+  }
+  arrive();
+  settle(qf);
+  settle(df);
   for (int it = 0; it < steps; ++it) {
     const int k0 = k_begin + it * KB, cur = it & 1;
     if (it + 1 < steps) fetch(k0 + KB, cur ^ 1);
@@ -706,7 +715,8 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
         float bend = 1.f;
         const float x =
             PLAIN ? __builtin_fmaf(p[r], a.c, -ls)
-                  : score(p[r], far + ((r & 3) + 8 * (r >> 2)), bend) - ls;
+                  : score(
+                        p[r], far + ((r & 3) + 8 * (r >> 2)), bend) - ls;
         dp[r] -= dl;
         if (CAP) dp[r] *= bend;
         dp[r] *= __builtin_amdgcn_exp2f(x);
@@ -864,27 +874,24 @@ __global__ __launch_bounds__(ST) void spans_kernel(
   y[3 * n] = e;
 }
 
-template <int D, bool CAP, bool BIAS>
+template <int D, bool CAP, bool BIAS, int NW, int KB>
 int launch_fwd(const Args& a, hipStream_t s) {
-  const int blocks = (a.S + 255) / 256, heads = a.B * a.H;
-  hipLaunchKernelGGL((fwd_kernel<D, CAP, BIAS>),
-                     dim3((unsigned)blocks * heads), dim3(512), 0, s, a, blocks,
-                     heads);
+  const int blocks = (a.S + 32 * NW - 1) / (32 * NW), heads = a.B * a.H;
+  hipLaunchKernelGGL((fwd_kernel<D, CAP, BIAS, NW, KB>),
+                     dim3((unsigned)blocks * heads), dim3(64 * NW), 0, s, a,
+                     blocks, heads);
   return (int)hipGetLastError();
 }
 
 template <int D, bool CAP, bool BIAS>
 int launch_bwd(const Args& a, int splits, hipStream_t s) {
-  const long long rows = (long long)a.B * a.S * a.H;
-  hipLaunchKernelGGL((stat_kernel<D>), dim3((unsigned)((rows + 15) / 16)),
-                     dim3(256), 0, s, a, rows);
   const int blocks = (a.S + 127) / 128;
-  hipLaunchKernelGGL((dkdv_kernel<D, CAP, BIAS>),
-                     dim3((unsigned)blocks * a.B * a.Hkv, splits), dim3(256),
-                     0, s, a, blocks, a.B * a.Hkv, rows);
   hipLaunchKernelGGL((dq_kernel<D, CAP, BIAS>),
                      dim3((unsigned)blocks * a.B * a.H), dim3(256), 0, s, a,
-                     blocks, a.B * a.H, rows);
+                     blocks, a.B * a.H);
+  hipLaunchKernelGGL((dkdv_kernel<D, CAP, BIAS>),
+                     dim3((unsigned)blocks * a.B * a.Hkv, splits), dim3(256),
+                     0, s, a, blocks, a.B * a.Hkv);
   if (splits > 1) {
     const long long n = (long long)a.B * a.S * a.Hkv * D;
     hipLaunchKernelGGL(add_kernel, dim3((unsigned)((2 * n / 4 + 255) / 256)),
@@ -896,8 +903,14 @@ int launch_bwd(const Args& a, int splits, hipStream_t s) {
 template <int D>
 int launch(const Args& a, int splits, hipStream_t s) {
   const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
-#define GO(C, W)                                    \
-  (splits ? launch_bwd<D, C, W>(a, splits, s) : launch_fwd<D, C, W>(a, s))
+  // Steps of 32 keys leave room for three workgroups a CU where heads of 96 and 128
+  // need registers for two otherwise (us, 64 / 32 keys: 1 x 8192 capped 811 / 769, nine
+  // documents in 4 x 4096 258 / 230, heads of 96 273 / 250); heads of 64 hold four
+  // either way (59 / 62). Eight waves that share the tiles took 883, 305, 296 and 64.
+  constexpr int KB = D == 64 ? 64 : 32;
+#define GO(C, W)                      \
+  (splits ? launch_bwd<D, C, W>(a, splits, s) \
+          : launch_fwd<D, C, W, 4, KB>(a, s))
   if (cap) return bias ? GO(true, true) : GO(true, false);
   return bias ? GO(false, true) : GO(false, false);
 #undef GO
