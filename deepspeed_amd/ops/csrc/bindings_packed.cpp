@@ -3,6 +3,9 @@
 
 #include "bindings.h"
 
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <tuple>
 
 extern "C" int ds_packed_spans(const void* ids, int wide, const int* prefix,
@@ -41,12 +44,35 @@ extern "C" int ds_logprobs_bwd(const void* x, long long outer_stride,
 namespace {
 
 using Opt = c10::optional<at::Tensor>;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 // Threads of a launch are counted in 32 bits.
 constexpr int64_t THREADS = 1ll << 32;
 
 void* data(const Opt& t) {
   return t.has_value() && t->defined() ? t->data_ptr() : nullptr;
+}
+
+Tensor or_none(const Opt& t) { return t.has_value() ? *t : Tensor(); }
+
+// The operators' autograd is here, not in Python: a backward pass of a few tens of us
+// waits as long again for the interpreter's lock in the engine's thread (a short
+// attention, there and back: 105 us so, 55 of them an empty Python function's).
+// Gradients have none of their own: a second derivative raises.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  const int64_t n = grads.size();
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " is differentiable once", n);
+  return node->apply(std::move(grads));
+}
+
+bool wants_grad(const Tensor& t) {
+  return at::GradMode::is_enabled() && t.requires_grad();
 }
 
 at::Tensor packed_spans(at::Tensor ids, Opt prefix, bool causal) {
@@ -112,8 +138,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_fwd(
     const int e = ds_masked_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
         lse.data_ptr<float>(), with_rest ? rest.data_ptr() : nullptr, nullptr,
-        nullptr, nullptr, nullptr, nullptr, nullptr, 0, a.spans, a.slopes, a.strides.data(), a.B, a.S, a.H, a.Hkv,
-        a.D, causal, (float)scale, (float)cap, cur_stream());
+        nullptr, nullptr, nullptr, nullptr, nullptr, 0, a.spans, a.slopes,
+        a.strides.data(), a.B, a.S, a.H, a.Hkv, a.D, causal, (float)scale, (float)cap, cur_stream());
     TORCH_CHECK(e == 0, "masked_attention: launch failed, hipError_t ", e);
   }
   return {o, lse, rest};
@@ -141,8 +167,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_bwd(
   if (q.numel()) {
     const int e = ds_masked_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-        lse.data_ptr<float>(), rest.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-        dv.data_ptr(), stat.data_ptr<float>(), part.data_ptr<float>(), splits,
+        lse.data_ptr<float>(), rest.data_ptr(), dout.data_ptr(), dq.data_ptr(),
+        dk.data_ptr(), dv.data_ptr(), stat.data_ptr<float>(), part.data_ptr<float>(), splits,
         a.spans, a.slopes, a.strides.data(), a.B, a.S, a.H, a.Hkv, a.D, causal,
         (float)scale, (float)cap, cur_stream());
     TORCH_CHECK(e == 0, "masked_attention: launch failed, hipError_t ", e);
@@ -150,12 +176,106 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_bwd(
   return {dq, dk, dv};
 }
 
+// x as the attention kernels read it: unit stride inside a head, 16-byte rows.
+Tensor rows_of(const Tensor& x) {
+  bool fits = x.stride(3) == 1 && (uintptr_t)x.data_ptr() % 16 == 0 &&
+              x.stride(1) < (1 << 24);
+  for (int d = 0; d < 3; ++d)
+    fits = fits && x.stride(d) % 8 == 0 && x.stride(d) >= 0;
+  return fits ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+struct MaskedAttention : torch::autograd::Function<MaskedAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_,
+                        const Tensor& v_, const Opt& spans,
+                        const Opt& slopes, bool causal, double scale,
+                        double cap, bool grads) {
+    // the kernels take maxima of scores that a positive scale has left in order
+    auto q = q_;
+    double factor = 1;
+    if (!(scale > 0)) {
+      factor = scale < 0 ? -1 : scale;
+      q = q * factor;
+      scale = scale < 0 ? -scale : 1;
+    }
+    q = rows_of(q);
+    const auto k = rows_of(k_), v = rows_of(v_);
+    auto [o, lse, rest] =
+        masked_attn_fwd(q, k, v, spans, slopes, causal, scale, cap, grads);
+    if (grads) {
+      ctx->save_for_backward({q, k, v, o, lse, rest, or_none(spans),
+                              or_none(slopes)});
+      ctx->saved_data["causal"] = causal;
+      ctx->saved_data["scale"] = scale;
+      ctx->saved_data["cap"] = cap;
+      ctx->saved_data["factor"] = factor;
+    }
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto t = ctx->get_saved_variables();
+    const double factor = ctx->saved_data["factor"].toDouble();
+    auto [dq, dk, dv] = masked_attn_bwd(
+        t[0], t[1], t[2], t[3], rows_of(g[0]), t[4], t[5], t[6], t[7],
+        ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble(),
+        ctx->saved_data["cap"].toDouble());
+    if (factor != 1) dq = dq * factor;
+    variable_list grads = once({dq, dk, dv}, "masked_attention");
+    grads.resize(9);
+    return grads;
+  }
+};
+
+Tensor masked_attention(const Tensor& q, const Tensor& k, const Tensor& v,
+                        const Opt& spans, const Opt& alibi_slopes, bool causal,
+                        c10::optional<double> scale, double softcap) {
+  TORCH_CHECK_VALUE(
+      q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() &&
+      q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+      q.size(3) == k.size(3) && k.size(2) > 0 && q.size(2) % k.size(2) == 0,
+      "masked_attention: q is [B, S, H, D], k and v are [B, S, Hkv, D] with H a "
+      "multiple of Hkv, got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+  TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type() &&
+                    q.scalar_type() == v.scalar_type(),
+                    "masked_attention: q, k and v of one type");
+  TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 &&
+                    (q.size(3) == 64 || q.size(3) == 96 || q.size(3) == 128),
+                    "masked_attention: bf16 and heads of 64, 96 or 128 on a GPU, "
+                    "got ", q.scalar_type(), " and ", q.size(3));
+  TORCH_CHECK_VALUE(softcap >= 0 && softcap < 1e30,
+                    "masked_attention: softcap is 0 (none) or positive, got ",
+                    softcap);
+  TORCH_CHECK_VALUE(!spans.has_value() ||
+                    (spans->dim() == 3 && spans->size(1) == q.size(0) &&
+                     spans->size(2) == q.size(1) && spans->device() == q.device()),
+                    "masked_attention: rows of another batch or device");
+  Opt slopes;
+  if (alibi_slopes.has_value()) {
+    const auto& t = *alibi_slopes;
+    TORCH_CHECK_VALUE(!t.requires_grad(),
+                      "masked_attention: alibi_slopes have no gradient");
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == q.size(2) &&
+                      t.is_floating_point(),
+                      "masked_attention: alibi_slopes is one number a query head");
+    TORCH_CHECK_VALUE(t.device() == q.device(),
+                      "masked_attention: tensors on different devices");
+    slopes = t.to(at::kFloat).contiguous();
+  }
+  TORCH_CHECK_VALUE(k.device() == q.device() && v.device() == q.device(),
+                    "masked_attention: tensors on different devices");
+  return MaskedAttention::apply(
+      q, k, v, spans, slopes, causal,
+      scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3)), softcap,
+      wants_grad(q) || wants_grad(k) || wants_grad(v));
+}
+
 // q [B, S, H, D], k [B, S, Hk, D], any strides but one inside a head; with dq and dk
 // the backward: (dq, dk, dwq, dwk) instead of (q, k).
-std::vector<at::Tensor> qk_norm_rope(at::Tensor q, at::Tensor k, at::Tensor wq,
-                                     at::Tensor wk, at::Tensor cs,
-                                     at::Tensor sn, Opt positions, double eps,
-                                     bool half, bool one_plus, Opt dq, Opt dk) {
+variable_list qk_norm_kernels(const Tensor& q, const Tensor& k, const Tensor& wq,
+                              const Tensor& wk, const Tensor& cs,
+                              const Tensor& sn, const Opt& positions,
+                              double eps, bool half, bool one_plus, Opt dq,
+                              Opt dk) {
   const OneDevice on("qk_norm_rope", q, k, wq, wk, cs, sn, positions, dq, dk);
   TORCH_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 &&
               q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
@@ -196,7 +316,7 @@ std::vector<at::Tensor> qk_norm_rope(at::Tensor q, at::Tensor k, at::Tensor wq,
   }
   auto yq = at::empty({B, S, H, D}, q.options());
   auto yk = at::empty({B, S, Hk, D}, q.options());
-  std::vector<at::Tensor> out = {yq, yk};
+  variable_list out = {yq, yk};
   const int parts = tokens ? ds_qk_norm_parts((int)tokens) : 0;
   at::Tensor part;
   if (back) {
@@ -218,13 +338,104 @@ std::vector<at::Tensor> qk_norm_rope(at::Tensor q, at::Tensor k, at::Tensor wq,
   return out;
 }
 
+Tensor inside(const Tensor& x) {     // unit stride inside a head
+  return x.stride(-1) == 1 ? x : x.contiguous();
+}
+
+struct QkNorm : torch::autograd::Function<QkNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q_,
+                               const Tensor& k_, const Tensor& wq_,
+                               const Tensor& wk_, const Tensor& cs,
+                               const Tensor& sn, const Opt& positions,
+                               double eps, bool half, bool one_plus) {
+    const auto q = inside(q_), k = inside(k_);
+    const auto wq = wq_.contiguous(), wk = wk_.contiguous();
+    auto out = qk_norm_kernels(q, k, wq, wk, cs, sn, positions, eps, half,
+                               one_plus, c10::nullopt, c10::nullopt);
+    ctx->save_for_backward({q, k, wq, wk, cs, sn, or_none(positions)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["half"] = half;
+    ctx->saved_data["one_plus"] = one_plus;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto t = ctx->get_saved_variables();
+    auto grads = once(
+        qk_norm_kernels(t[0], t[1], t[2], t[3], t[4], t[5], t[6],
+                        ctx->saved_data["eps"].toDouble(),
+                        ctx->saved_data["half"].toBool(),
+                        ctx->saved_data["one_plus"].toBool(), inside(g[0]),
+                        inside(g[1])), "qk_norm_rope");
+    grads.resize(10);
+    return grads;
+  }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
+                                        const Tensor& q_weight,
+                                        const Tensor& k_weight,
+                                        const Tensor& cos, const Tensor& sin,
+                                        const Opt& positions, double eps,
+                                        bool half, bool one_plus) {
+  const int64_t D = q.dim() ? q.size(-1) : 0;
+  TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) &&
+                    q.size(1) == k.size(1) && k.size(3) == D && D % 2 == 0 &&
+                    D >= 2 && D <= 512,
+                    "qk_norm_rope: q is [B, S, H, D], k [B, S, Hk, D], D even and "
+                    "up to 512, got ", q.sizes(), " and ", k.sizes());
+  TORCH_CHECK_VALUE(q_weight.dim() == 1 && q_weight.size(0) == D &&
+                    k_weight.dim() == 1 && k_weight.size(0) == D,
+                    "qk_norm_rope: weights are [D]");
+  const auto type = q.scalar_type();
+  TORCH_CHECK_VALUE(type == k.scalar_type() && type == q_weight.scalar_type() &&
+                    type == k_weight.scalar_type(),
+                    "qk_norm_rope: heads and weights of one type, got ", type,
+                    ", ", k.scalar_type(), ", ", q_weight.scalar_type(), ", ",
+                    k_weight.scalar_type());
+  TORCH_CHECK_VALUE(type == at::kBFloat16 || type == at::kHalf ||
+                    type == at::kFloat,
+                    "qk_norm_rope: bf16, fp16 or fp32 on a GPU");
+  TORCH_CHECK_VALUE(cos.dim() == 2 && cos.sizes() == sin.sizes() &&
+                    cos.size(1) >= 1 && 2 * cos.size(1) <= D &&
+                    cos.scalar_type() == at::kFloat &&
+                    sin.scalar_type() == at::kFloat,
+                    "qk_norm_rope: cos and sin are fp32 [positions, rotated / 2]");
+  TORCH_CHECK_VALUE(!positions.has_value() ||
+                    (positions->scalar_type() == at::kInt &&
+                     positions->numel() == q.size(0) * q.size(1)),
+                    "qk_norm_rope: positions are int32, one a token");
+  TORCH_CHECK_VALUE(positions.has_value() || q.size(1) <= cos.size(0),
+                    "qk_norm_rope: rows longer than the tables");
+  bool here = true;
+  for (const auto* t : {&k, &q_weight, &k_weight, &cos, &sin})
+    here = here && t->device() == q.device();
+  TORCH_CHECK_VALUE(here && (!positions.has_value() ||
+                             positions->device() == q.device()),
+                    "qk_norm_rope: tensors on different devices");
+  Opt pos;
+  if (positions.has_value()) pos = positions->contiguous();
+  const auto c = cos.contiguous(), s = sin.contiguous();
+  if (wants_grad(q) || wants_grad(k) || wants_grad(q_weight) ||
+      wants_grad(k_weight)) {
+    const auto y = QkNorm::apply(q, k, q_weight, k_weight, c, s, pos, eps, half,
+                                 one_plus);
+    return {y[0], y[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto y = qk_norm_kernels(inside(q), inside(k), q_weight.contiguous(),
+                                 k_weight.contiguous(), c, s, pos, eps, half,
+                                 one_plus, c10::nullopt, c10::nullopt);
+  return {y[0], y[1]};
+}
+
 // Logits as rows of two strides: [V], [N, V] or [B, S, V], unit stride inside.
 struct LogitRows {
   int64_t rows = 1, V, inner = 1, outer_stride = 0, inner_stride = 0;
   int type;
   LogitRows(const at::Tensor& x, const at::Tensor& tokens) {
     const int64_t n = x.dim();
-    TORCH_CHECK(x.is_cuda() && n >= 1 && n <= 3 && x.stride(n - 1) == 1,
+    TORCH_CHECK(x.is_cuda() && n >= 1 && n <= 3 &&
+                (x.stride(n - 1) == 1 || x.size(n - 1) == 1),
                 "token_logprobs: logits [.., V], unit stride inside");
     V = x.size(n - 1);
     if (n == 3) {
@@ -244,8 +455,8 @@ struct LogitRows {
   }
 };
 
-std::vector<at::Tensor> logprobs_fwd(at::Tensor x, at::Tensor tokens,
-                                     int64_t top, int64_t ignore) {
+variable_list logprobs_fwd(const Tensor& x, const Tensor& tokens, int64_t top,
+                           int64_t ignore) {
   const OneDevice on("token_logprobs", x, tokens);
   const LogitRows r(x, tokens);
   const int parts = ds_logprobs_parts((int)r.rows, r.V, (int)top);
@@ -253,10 +464,11 @@ std::vector<at::Tensor> logprobs_fwd(at::Tensor x, at::Tensor tokens,
               "token_logprobs: up to 32 of up to 500000 tokens");
   TORCH_CHECK(r.rows * (parts + 1) * 256 < THREADS, "token_logprobs: size");
   const auto f32 = x.options().dtype(at::kFloat);
-  auto lp = at::empty({r.rows}, f32), ent = at::empty({r.rows}, f32);
+  auto lp = at::empty(tokens.sizes(), f32), ent = at::empty(tokens.sizes(), f32);
   auto stat = at::empty({r.rows, 2}, f32);
-  auto top_lp = at::empty({r.rows, top}, f32);
-  auto ids = at::empty({r.rows, top}, tokens.options());
+  auto best = tokens.sizes().vec();
+  best.push_back(top);
+  auto top_lp = at::empty(best, f32), ids = at::empty(best, tokens.options());
   if (r.rows) {
     // the parts' sums, then on 8 bytes the waves' lists
     const int64_t of_sums = (r.rows * parts * 3 + 1) / 2 * 2;
@@ -299,23 +511,79 @@ at::Tensor logprobs_bwd(at::Tensor x, at::Tensor tokens, at::Tensor stat,
   return dx;
 }
 
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits,
+                               const Tensor& tokens, int64_t top,
+                               int64_t ignore) {
+    // up to three dimensions of any strides but one inside a row
+    auto x = logits;
+    if (x.dim() > 3) x = x.reshape({-1, x.size(-2), x.size(-1)});
+    if (x.size(-1) > 1 && x.stride(-1) != 1) x = x.contiguous();
+    auto out = logprobs_fwd(x, tokens, top, ignore);
+    ctx->save_for_backward({x, tokens, out[2], out[1]});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->mark_non_differentiable({out[3], out[4]});
+    ctx->set_materialize_grads(false);
+    return {out[0], out[1], out[3], out[4]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list grads(4);
+    if (!g[0].defined() && !g[1].defined()) return grads;
+    const auto t = ctx->get_saved_variables();
+    for (int i = 0; i < 2; ++i)
+      if (g[i].defined()) g[i] = g[i].to(at::kFloat).contiguous();
+    auto shape = t[1].sizes().vec();
+    shape.push_back(t[0].size(-1));
+    auto dx = logprobs_bwd(t[0], t[1], t[2], t[3], g[0], g[1],
+                           ctx->saved_data["ignore"].toInt());
+    grads[0] = once({dx.view(shape)}, "token_logprobs")[0];
+    return grads;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(
+    const Tensor& logits, const Tensor& tokens, int64_t top,
+    int64_t ignore_index) {
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 &&
+                    logits.sizes().slice(0, logits.dim() - 1) == tokens.sizes(),
+                    "token_logprobs: logits [.., V] and tokens [..], got ",
+                    logits.sizes(), " and ", tokens.sizes());
+  TORCH_CHECK_VALUE(tokens.scalar_type() == at::kInt ||
+                    tokens.scalar_type() == at::kLong,
+                    "token_logprobs: integer tokens, got ", tokens.scalar_type());
+  const auto type = logits.scalar_type();
+  TORCH_CHECK_VALUE(type == at::kBFloat16 || type == at::kHalf ||
+                    type == at::kFloat,
+                    "token_logprobs: floating logits, bf16, fp16 or fp32 on a "
+                    "GPU, got ", type);
+  const int64_t V = logits.size(-1);
+  TORCH_CHECK_VALUE(top >= 0 && top <= 32 && top <= V &&
+                    (top == 0 || V <= 500000),
+                    "token_logprobs: up to 32 best of 500000 tokens at most, got ",
+                    top, " of ", V);
+  TORCH_CHECK_VALUE(logits.device() == tokens.device(),
+                    "token_logprobs: tensors on different devices");
+  const auto y = TokenLogprobs::apply(
+      logits, tokens.to(at::kLong).contiguous(), top, ignore_index);
+  return {y[0], y[1], y[2], y[3]};
+}
+
 }  // namespace
 
 void bind_packed(pybind11::module_& m) {
   namespace py = pybind11;
   m.def("packed_spans", &packed_spans,
         "the keys that each query sees, the queries that see each key");
-  m.def("masked_attn_fwd", &masked_attn_fwd,
-        "attention over packed rows: (o, logsumexp, what o was rounded by)");
-  m.def("masked_attn_bwd", &masked_attn_bwd,
-        "its backward: (dq, dk, dv)");
-  m.def("qk_norm_rope", &qk_norm_rope,
-        "norms and rotation of queries and keys, or their backward",
-        py::arg("q"), py::arg("k"), py::arg("wq"), py::arg("wk"), py::arg("cos"),
-        py::arg("sin"), py::arg("positions"), py::arg("eps"), py::arg("half"),
-        py::arg("one_plus"), py::arg("dq") = c10::nullopt,
-        py::arg("dk") = c10::nullopt);
-  m.def("logprobs_fwd", &logprobs_fwd,
-        "log probabilities, entropy and best tokens of rows of logits");
-  m.def("logprobs_bwd", &logprobs_bwd, "gradient of the logits");
+  m.def("masked_attention", &masked_attention, "attention over packed rows",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("spans"),
+        py::arg("alibi_slopes"), py::arg("causal"), py::arg("scale"),
+        py::arg("softcap"));
+  m.def("qk_norm_rope", &qk_norm_rope, "norms and rotation of queries and keys",
+        py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"),
+        py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("eps"),
+        py::arg("half"), py::arg("one_plus"));
+  m.def("token_logprobs", &token_logprobs,
+        "log probabilities, entropy and best tokens of rows of logits",
+        py::arg("logits"), py::arg("tokens"), py::arg("top"),
+        py::arg("ignore_index"));
 }

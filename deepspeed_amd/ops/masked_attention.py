@@ -11,7 +11,6 @@ from typing import Optional
 import torch
 
 from ._loader import get_ext
-from .attention import _rows, _scaled
 from .linear import untransformed
 
 
@@ -103,29 +102,6 @@ def _torch_attention(q, k, v, spans, causal, scale, softcap, slopes):
     return (p @ vt).transpose(1, 2).to(q.dtype)
 
 
-class _MaskedAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, spans, slopes, causal, scale, softcap):
-        q, scale, ctx.factor = _scaled(q, scale)
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        o, lse, rest = get_ext().masked_attn_fwd(
-            q, k, v, spans, slopes, causal, scale, softcap,
-            any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, o, lse, rest, spans, slopes)
-        ctx.causal, ctx.scale, ctx.softcap = causal, scale, softcap
-        return o
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, do):
-        q, k, v, o, lse, rest, spans, slopes = ctx.saved_tensors
-        dq, dk, dv = get_ext().masked_attn_bwd(
-            q, k, v, o, _rows(do), lse, rest, spans, slopes, ctx.causal, ctx.scale,
-            ctx.softcap)
-        dq = dq if ctx.factor == 1 else dq * ctx.factor
-        return dq, dk, dv, None, None, None, None, None
-
-
 def _checked_slopes(alibi_slopes, q, what):
     if alibi_slopes is None:
         return None
@@ -157,6 +133,11 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     query and key, softmax over the keys that a query sees: those of ``rows``, or
     without them by ``causal`` all up to its own or all there are. A query that sees
     none gives 0 and has no gradient. On a GPU bf16 and heads of 64, 96 or 128."""
+    ext = get_ext()
+    if q.is_cuda and ext is not None and untransformed():
+        spans, causal = (None, causal) if rows is None else (rows.spans, rows.causal)
+        return ext.masked_attention(q, k, v, spans, alibi_slopes, causal, scale,
+                                    softcap or 0.0)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or \
             q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or \
             k.shape[2] == 0 or q.shape[2] % k.shape[2]:
@@ -172,10 +153,5 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     softcap = _checked_cap(softcap, "masked_attention")
     slopes = _checked_slopes(alibi_slopes, q, "masked_attention")
     spans, causal = (rows.spans, rows.causal) if rows is not None else (None, causal)
-    if not q.is_cuda or get_ext() is None or not untransformed():
-        scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[3])
-        return _torch_attention(q, k, v, spans, causal, scale, softcap, slopes)
-    if q.dtype is not torch.bfloat16 or q.shape[3] not in (64, 96, 128):
-        raise ValueError("masked_attention: bf16 and heads of 64, 96 or 128 on a GPU, "
-                         f"got {q.dtype} and {q.shape[3]}")
-    return _MaskedAttentionFn.apply(q, k, v, spans, slopes, causal, scale, softcap)
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[3])
+    return _torch_attention(q, k, v, spans, causal, scale, softcap, slopes)

@@ -36,30 +36,6 @@ def _torch_heads(x, weight, cos, sin, positions, eps, layout, one_plus):
     return torch.cat([turned, y[..., n:]], -1).to(x.dtype)
 
 
-def _inside(x):
-    """x with unit stride inside a head, as the kernels read it."""
-    return x if x.stride(-1) == 1 else x.contiguous()
-
-
-class _HeadsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, half,
-                one_plus):
-        q, k = _inside(q), _inside(k)
-        yq, yk = get_ext().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions,
-                                        eps, half, one_plus)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.how = eps, half, one_plus
-        return yq, yk
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dq, dk):
-        grads = get_ext().qk_norm_rope(*ctx.saved_tensors, *ctx.how, _inside(dq),
-                                       _inside(dk))
-        return (*grads, None, None, None, None, None, None)
-
-
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
                  k_weight: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                  positions: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -75,6 +51,10 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     weights. bf16, fp16 or fp32, even D up to 512, all in fp32 and rounded once."""
     if layout not in LAYOUTS:
         raise ValueError(f"qk_norm_rope: layout is one of {LAYOUTS}, got {layout!r}")
+    ext = get_ext()
+    if q.is_cuda and ext is not None and untransformed():
+        return ext.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps,
+                                layout == "half", one_plus)
     D = q.shape[-1] if q.dim() else 0
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or \
             k.shape[3] != D or D % 2 or not 2 <= D <= 512:
@@ -98,12 +78,5 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     if any(t is not None and t.device != q.device
            for t in (k, q_weight, k_weight, cos, sin, positions)):
         raise ValueError("qk_norm_rope: tensors on different devices")
-    if not q.is_cuda or get_ext() is None or not untransformed():
-        how = cos, sin, positions, eps, layout, one_plus
-        return _torch_heads(q, q_weight, *how), _torch_heads(k, k_weight, *how)
-    if q.dtype is torch.float64:
-        raise ValueError("qk_norm_rope: bf16, fp16 or fp32 on a GPU")
-    return _HeadsFn.apply(q, k, q_weight.contiguous(), k_weight.contiguous(),
-                          cos.contiguous(), sin.contiguous(),
-                          None if positions is None else positions.contiguous(), eps,
-                          layout == "half", one_plus)
+    how = cos, sin, positions, eps, layout, one_plus
+    return _torch_heads(q, q_weight, *how), _torch_heads(k, k_weight, *how)

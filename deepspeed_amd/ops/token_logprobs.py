@@ -50,41 +50,6 @@ def _torch_logprobs(logits, tokens, top, ignore_index):
                          torch.where(live[..., None], order, -1))
 
 
-def _as_rows(logits):
-    """Logits as the kernels read them: up to three dimensions of any strides but one
-    inside a row."""
-    if logits.dim() > 3:
-        logits = logits.reshape(-1, logits.shape[-2], logits.shape[-1])
-    if logits.shape[-1] > 1 and logits.stride(-1) != 1:
-        logits = logits.contiguous()
-    return logits
-
-
-class _LogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top, ignore_index):
-        x = _as_rows(logits)
-        lp, entropy, stat, top_lp, top_ids = get_ext().logprobs_fwd(
-            x, tokens, top, ignore_index)
-        ctx.save_for_backward(x, tokens, stat, entropy)
-        ctx.shape, ctx.ignore_index = logits.shape, ignore_index
-        ctx.mark_non_differentiable(top_lp, top_ids)
-        ctx.set_materialize_grads(False)
-        return lp, entropy, top_lp, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, glp, gent, _top_lp, _top_ids):
-        if glp is None and gent is None:
-            return None, None, None, None
-        x, tokens, stat, entropy = ctx.saved_tensors
-        glp, gent = (None if g is None else g.float().contiguous()
-                     for g in (glp, gent))
-        dx = get_ext().logprobs_bwd(x, tokens, stat, entropy, glp, gent,
-                                    ctx.ignore_index)
-        return dx.view(ctx.shape), None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
                    ignore_index: int = -100) -> TokenLogprobs:
     """``logits`` [.., V] bf16, fp16 or fp32 and ``tokens`` [..] (integers) -> the log
@@ -93,6 +58,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     (once) in the logits through ``logprobs`` and ``entropy``. Tokens of
     ``ignore_index`` give 0 and 0, no gradient, and ids of -1; a token that is not in
     the vocabulary gives NaN, and a NaN logit counts above all others."""
+    ext = get_ext()
+    if logits.is_cuda and ext is not None and untransformed():
+        return TokenLogprobs(*ext.token_logprobs(logits, tokens, top, ignore_index))
     if logits.dim() < 1 or logits.shape[:-1] != tokens.shape or logits.shape[-1] < 1:
         raise ValueError("token_logprobs: logits [.., V] and tokens [..], got "
                          f"{tuple(logits.shape)} and {tuple(tokens.shape)}")
@@ -107,12 +75,4 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
                          f"most, got {top} of {V}")
     if logits.device != tokens.device:
         raise ValueError("token_logprobs: tensors on different devices")
-    tokens = tokens.long().contiguous()
-    if not logits.is_cuda or get_ext() is None or not untransformed():
-        return _torch_logprobs(logits, tokens, top, ignore_index)
-    if logits.dtype is torch.float64:
-        raise ValueError("token_logprobs: bf16, fp16 or fp32 on a GPU")
-    lp, entropy, top_lp, top_ids = _LogprobsFn.apply(logits, tokens, top, ignore_index)
-    shape = tokens.shape
-    return TokenLogprobs(lp.view(shape), entropy.view(shape),
-                         top_lp.view(*shape, top), top_ids.view(*shape, top))
+    return _torch_logprobs(logits, tokens.long(), top, ignore_index)

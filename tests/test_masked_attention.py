@@ -565,3 +565,22 @@ def test_decode_bad_pages_gpu(bs):
                        paged_decode_attention(q, kp, vp, table, most, softcap=10.0))
     with pytest.raises(ValueError, match="up to 16 a key head"):
         paged_decode_attention(q.float(), kp, vp, table, n, softcap=1.0)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_raise_gpu():
+    """Gradients that a graph is asked for say so when they are differentiated, and
+    are the same until then."""
+    q, k, v, do = _inputs(1, 9, 2, 1, 64, "cuda")
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    plain = torch.autograd.grad(masked_attention(*leaves), leaves, do)
+    o = masked_attention(*leaves)
+    graph = torch.autograd.grad(o, leaves, do, create_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(plain, graph))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        graph[0].float().sum().backward()
+    # only the gradient that is asked for, by other types of a call
+    dv, = torch.autograd.grad(masked_attention(q, k, leaves[2]), leaves[2], do)
+    assert torch.equal(dv, plain[2])
+    with torch.no_grad():
+        assert not masked_attention(*leaves).requires_grad
