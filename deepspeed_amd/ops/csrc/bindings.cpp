@@ -109,13 +109,6 @@ extern "C" int ds_paged_rows(const void* q, const void* kpool,
                               int n_merges, int any_merge, int nq, int H,
                               int Hkv, int BS, int max_blocks, int splits,
                               float scale, void* stream);
-extern "C" int ds_paged_shaped(const void* q, const void* kpool,
-                               const void* vpool, const int* table,
-                               const int* lens, const float* slopes, void* out,
-                               float* part, float* part_ml, int n, int H,
-                               int Hkv, int BS, int max_blocks, int blocks,
-                               int splits, float scale, float cap,
-                               void* stream);
 extern "C" int ds_rows_linear(const void* x, int layers, const void* const* w,
                               const float* const* scales,
                               const void* const* bias, void* const* out,
@@ -373,10 +366,8 @@ static void check_pool(const at::Tensor& q, const at::Tensor& kpool,
 
 at::Tensor paged_decode(at::Tensor q, at::Tensor kpool, at::Tensor vpool,
                         at::Tensor block_table, at::Tensor lens,
-                        int64_t splits, double scale, double softcap,
-                        c10::optional<at::Tensor> slopes) {
-  const OneDevice on("paged_decode", q, kpool, vpool, block_table, lens,
-                     slopes);
+                        int64_t splits, double scale) {
+  const OneDevice on("paged_decode", q, kpool, vpool, block_table, lens);
   check_pool(q, kpool, vpool, "paged_decode");
   const int n = q.size(0), H = q.size(1);
   const int Hkv = kpool.size(1), BS = kpool.size(2);
@@ -394,24 +385,6 @@ at::Tensor paged_decode(at::Tensor q, at::Tensor kpool, at::Tensor vpool,
   auto part_ml = at::empty({splits > 1 ? items * Hkv * 16 * 2 : 0}, f32);
   auto o = at::empty_like(q);
   if (n == 0) return o;
-  if (softcap > 0 || slopes.has_value()) {
-    TORCH_CHECK(softcap >= 0 && softcap < 1e30, "paged_decode: softcap");
-    TORCH_CHECK(!slopes.has_value() ||
-                (slopes->scalar_type() == at::kFloat &&
-                 slopes->is_contiguous() && slopes->numel() == H),
-                "paged_decode: alibi_slopes fp32 [H]");
-    TORCH_CHECK(kpool.size(0) > 0 && kpool.size(0) < (1ll << 31) &&
-                items * 256 < (1ll << 32), "paged_decode: size");
-    const int e = ds_paged_shaped(
-        q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(),
-        block_table.data_ptr<int>(), lens.data_ptr<int>(),
-        slopes.has_value() ? slopes->data_ptr<float>() : nullptr, o.data_ptr(),
-        part.data_ptr<float>(), part_ml.data_ptr<float>(), n, H, Hkv, BS,
-        (int)block_table.size(1), (int)kpool.size(0), (int)splits,
-        (float)scale, (float)softcap, cur_stream());
-    TORCH_CHECK(e == 0, "paged_decode: launch failed, hipError_t ", e);
-    return o;
-  }
   const int e = ds_paged_rows(
       q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(),
       block_table.data_ptr<int>(), nullptr, nullptr, nullptr,
@@ -1494,12 +1467,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(pybind11::init<const std::string&, int64_t, int64_t, int64_t>())
       .def("all_reduce", &ShmComm::all_reduce);
   m.def("paged_decode", &paged_decode,
-        "split-KV decode attention over a paged KV block table",
-        pybind11::arg("q"), pybind11::arg("kpool"), pybind11::arg("vpool"),
-        pybind11::arg("block_table"), pybind11::arg("lens"),
-        pybind11::arg("splits"), pybind11::arg("scale"),
-        pybind11::arg("softcap") = 0.0,
-        pybind11::arg("alibi_slopes") = c10::nullopt);
+        "split-KV decode attention over a paged KV block table");
   m.def("rows_linear", &rows_linear,
         "linear layers of a few rows, bf16 or groupwise int8 weights");
   m.def("tile_linear", &tile_linear, "linear layers of many rows, bf16",

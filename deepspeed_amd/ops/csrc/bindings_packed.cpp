@@ -1,11 +1,13 @@
-// Python bindings of the operators for packed rows: masked attention, the norms and
-// rotation of queries and keys, log probabilities of tokens.
+// Python bindings of the operators for packed rows: masked attention and its form for
+// single tokens, the norms and rotation of queries and keys, log probabilities.
 
 #include "bindings.h"
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
+#include <cmath>
 #include <tuple>
 
 extern "C" int ds_packed_spans(const void* ids, int wide, const int* prefix,
@@ -17,6 +19,13 @@ extern "C" int ds_masked_attention(
     float* part, int splits, const int* spans, const float* slopes,
     const long long* strides, int B, int S, int H, int Hkv, int D, int causal,
     float scale, float cap, void* stream);
+extern "C" int ds_paged_shaped(const void* q, const void* kpool,
+                               const void* vpool, const int* table,
+                               const int* lens, const float* slopes, void* out,
+                               float* part, float* part_ml, int n, int H,
+                               int Hkv, int BS, int max_blocks, int blocks,
+                               int splits, float scale, float cap,
+                               void* stream);
 extern "C" int ds_flash_bwd_splits(int B, int S, int H, int Hkv);
 extern "C" int ds_qk_norm_parts(int tokens);
 extern "C" int ds_qk_norm_rope(
@@ -226,6 +235,23 @@ struct MaskedAttention : torch::autograd::Function<MaskedAttention> {
   }
 };
 
+Opt slopes_of(const Opt& t, const Tensor& q, const char* what) {
+  if (!t.has_value()) return t;
+  TORCH_CHECK_VALUE(!t->requires_grad(), what, ": alibi_slopes have no gradient");
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == q.size(-2) &&
+                    t->is_floating_point(),
+                    what, ": alibi_slopes is one number a query head, got ",
+                    t->sizes());
+  TORCH_CHECK_VALUE(t->device() == q.device(),
+                    what, ": tensors on different devices");
+  return t->to(at::kFloat).contiguous();
+}
+
+void check_cap(double softcap, const char* what) {
+  TORCH_CHECK_VALUE(softcap >= 0 && softcap < 1e30, what,
+                    ": softcap is 0 (none) or positive, got ", softcap);
+}
+
 Tensor masked_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                         const Opt& spans, const Opt& alibi_slopes, bool causal,
                         c10::optional<double> scale, double softcap) {
@@ -242,31 +268,88 @@ Tensor masked_attention(const Tensor& q, const Tensor& k, const Tensor& v,
                     (q.size(3) == 64 || q.size(3) == 96 || q.size(3) == 128),
                     "masked_attention: bf16 and heads of 64, 96 or 128 on a GPU, "
                     "got ", q.scalar_type(), " and ", q.size(3));
-  TORCH_CHECK_VALUE(softcap >= 0 && softcap < 1e30,
-                    "masked_attention: softcap is 0 (none) or positive, got ",
-                    softcap);
+  check_cap(softcap, "masked_attention");
   TORCH_CHECK_VALUE(!spans.has_value() ||
                     (spans->dim() == 3 && spans->size(1) == q.size(0) &&
                      spans->size(2) == q.size(1) && spans->device() == q.device()),
                     "masked_attention: rows of another batch or device");
-  Opt slopes;
-  if (alibi_slopes.has_value()) {
-    const auto& t = *alibi_slopes;
-    TORCH_CHECK_VALUE(!t.requires_grad(),
-                      "masked_attention: alibi_slopes have no gradient");
-    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == q.size(2) &&
-                      t.is_floating_point(),
-                      "masked_attention: alibi_slopes is one number a query head");
-    TORCH_CHECK_VALUE(t.device() == q.device(),
-                      "masked_attention: tensors on different devices");
-    slopes = t.to(at::kFloat).contiguous();
-  }
+  const Opt slopes = slopes_of(alibi_slopes, q, "masked_attention");
   TORCH_CHECK_VALUE(k.device() == q.device() && v.device() == q.device(),
                     "masked_attention: tensors on different devices");
   return MaskedAttention::apply(
       q, k, v, spans, slopes, causal,
       scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3)), softcap,
       wants_grad(q) || wants_grad(k) || wants_grad(v));
+}
+
+Tensor aligned(const Tensor& t) {     // contiguous, on 16 bytes
+  const auto x = t.contiguous();
+  return (uintptr_t)x.data_ptr() % 16 == 0 ? x : x.clone();
+}
+
+// splits 0: by sizes.
+Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
+                    const Tensor& vpool_, const Tensor& table_,
+                    const Tensor& lens_, int64_t splits,
+                    c10::optional<double> scale, double softcap,
+                    const Opt& alibi_slopes) {
+  const char* what = "paged_decode_attention";
+  TORCH_CHECK_VALUE(q_.dim() == 3 && kpool_.dim() == 4 &&
+                    kpool_.sizes() == vpool_.sizes() &&
+                    q_.size(2) == kpool_.size(3) && kpool_.size(1) > 0 &&
+                    q_.size(1) % kpool_.size(1) == 0 && kpool_.size(2) > 0,
+                    what, ": q is [n, H, D], the pools are [blocks, Hkv, BS, D] "
+                    "with H a multiple of Hkv, got ", q_.sizes(), ", ",
+                    kpool_.sizes(), ", ", vpool_.sizes());
+  TORCH_CHECK_VALUE(table_.dim() == 2 && table_.size(0) == q_.size(0) &&
+                    lens_.dim() == 1 && lens_.size(0) == q_.size(0),
+                    what, ": block_table is [n, blocks], lens [n]");
+  TORCH_CHECK_VALUE(q_.scalar_type() == at::kBFloat16 &&
+                    kpool_.scalar_type() == at::kBFloat16 &&
+                    vpool_.scalar_type() == at::kBFloat16 &&
+                    q_.size(2) == 128 && q_.size(1) <= 16 * kpool_.size(1),
+                    what, ": bf16, heads of 128 and up to 16 a key head on a GPU");
+  bool here = true;
+  for (const auto* t : {&kpool_, &vpool_, &table_, &lens_})
+    here = here && t->device() == q_.device();
+  TORCH_CHECK_VALUE(here, what, ": tensors on different devices");
+  check_cap(softcap, what);
+  const Opt slopes = slopes_of(alibi_slopes, q_, what);
+  const OneDevice on(what, q_);
+  const auto q = aligned(q_), kpool = aligned(kpool_), vpool = aligned(vpool_);
+  const auto table = table_.to(at::kInt).contiguous();
+  const auto lens = lens_.to(at::kInt).contiguous();
+  const int64_t n = q.size(0), H = q.size(1), Hkv = kpool.size(1);
+  const int64_t BS = kpool.size(2), groups = n * Hkv;
+  auto o = at::empty_like(q);
+  if (n == 0) return o;
+  if (splits == 0) {
+    // One launch up to 1024 keys a request, which the table's width bounds (us, whole
+    // / cut for 1024 workgroups and merged: 1 x 700, 8 key heads 11.5 / 13.8; 32 x 700
+    // 14.2 / 19.7). Longer ones in parts of 500 keys and more: few requests for a
+    // workgroup a CU (9 x 4000 25.4 / 26.2, 9 x 12000 60.5 / 70.6), many for up to
+    // twelve (48 x 4000 87 / 92, 40 x 4000 71 / 73, 136 groups of 12000 97 / 104).
+    const int64_t keys = table.size(1) * BS;
+    splits = keys <= 1024 ? 1 : 2 * groups <= 256 ? 256 / groups : 3072 / groups;
+    splits = std::max<int64_t>(1, std::min({splits, keys / 500, (int64_t)32}));
+  }
+  TORCH_CHECK_VALUE(splits >= 1 && kpool.size(0) > 0 &&
+                    kpool.size(0) < (1ll << 31) && H * 128 < (1ll << 31) &&
+                    n * splits * 512 < THREADS && Hkv <= 65535 &&
+                    BS < (1ll << 31) && table.size(1) < (1ll << 31),
+                    what, ": size");
+  const int64_t items = splits > 1 ? n * splits * Hkv * 16 : 0;
+  auto part = at::empty({items * 130}, q.options().dtype(at::kFloat));
+  float* p = part.data_ptr<float>();
+  const int e = ds_paged_shaped(
+      q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), table.data_ptr<int>(),
+      lens.data_ptr<int>(), static_cast<const float*>(data(slopes)),
+      o.data_ptr(), p, p + items * 128, (int)n, (int)H, (int)Hkv, (int)BS,
+      (int)table.size(1), (int)kpool.size(0), (int)splits,
+      (float)(scale.has_value() ? *scale : 1.0 / std::sqrt(128.0)),
+      (float)softcap, cur_stream());
+  TORCH_CHECK(e == 0, what, ": launch failed, hipError_t ", e);
+  return o;
 }
 
 // q [B, S, H, D], k [B, S, Hk, D], any strides but one inside a head; with dq and dk
@@ -322,9 +405,9 @@ variable_list qk_norm_kernels(const Tensor& q, const Tensor& k, const Tensor& wq
   if (back) {
     out.push_back(tokens ? at::empty_like(wq) : at::zeros_like(wq));
     out.push_back(tokens ? at::empty_like(wk) : at::zeros_like(wk));
-    part = at::empty({parts, 2, D}, q.options().dtype(at::kFloat));
+    part = at::empty({parts, D}, q.options().dtype(at::kFloat));
   }
-  if (tokens == 0 || H + Hk == 0) return out;
+  if (tokens == 0) return out;
   const int e = ds_qk_norm_rope(
       q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), data(dq),
       data(dk), wq.data_ptr(), wk.data_ptr(), cs.data_ptr<float>(),
@@ -380,7 +463,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
   const int64_t D = q.dim() ? q.size(-1) : 0;
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) &&
                     q.size(1) == k.size(1) && k.size(3) == D && D % 2 == 0 &&
-                    D >= 2 && D <= 512,
+                    D >= 2 && D <= 512 && q.size(2) > 0 && k.size(2) > 0,
                     "qk_norm_rope: q is [B, S, H, D], k [B, S, Hk, D], D even and "
                     "up to 512, got ", q.sizes(), " and ", k.sizes());
   TORCH_CHECK_VALUE(q_weight.dim() == 1 && q_weight.size(0) == D &&
@@ -578,6 +661,11 @@ void bind_packed(pybind11::module_& m) {
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("spans"),
         py::arg("alibi_slopes"), py::arg("causal"), py::arg("scale"),
         py::arg("softcap"));
+  m.def("paged_shaped", &paged_shaped,
+        "attention of single tokens over the paged pool, scores shaped",
+        py::arg("q"), py::arg("kpool"), py::arg("vpool"), py::arg("block_table"),
+        py::arg("lens"), py::arg("splits"), py::arg("scale"), py::arg("softcap"),
+        py::arg("alibi_slopes"));
   m.def("qk_norm_rope", &qk_norm_rope, "norms and rotation of queries and keys",
         py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"),
         py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("eps"),

@@ -67,15 +67,48 @@ struct Sums {
   }
 };
 
-// Of the lanes `width` apart and nearer: the sums as if one had seen all.
+// Over the 64 lanes by moves inside the vector unit: rows of 16, the rows of a half,
+// the halves; the last lane has it all. Six exchanges through LDS take as long as
+// thirty of these, and a best token takes one or two such reductions.
+template <typename Op>
+__device__ __forceinline__ int over_lanes(int x, int none, Op op) {
+#define STEP(CTRL, ROWS) \
+  x = op(x, __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false))
+  STEP(0x111, 0xf);      // one lane up, two, four, eight
+  STEP(0x112, 0xf);
+  STEP(0x114, 0xf);
+  STEP(0x118, 0xf);
+  STEP(0x142, 0xa);      // a row's last lane to the next row
+  STEP(0x143, 0xc);      // the first half's to the second
+#undef STEP
+  return __builtin_amdgcn_readlane(x, 63);
+}
+__device__ __forceinline__ float as_float(int x) {
+  return __builtin_bit_cast(float, x);
+}
+__device__ __forceinline__ int as_int(float x) {
+  return __builtin_bit_cast(int, x);
+}
+__device__ __forceinline__ float lanes_max(float x) {
+  return as_float(over_lanes(as_int(x), as_int(LOWEST), [](int a, int b) {
+    return as_int(fmaxf(as_float(a), as_float(b)));
+  }));
+}
+__device__ __forceinline__ float lanes_sum(float x) {
+  return as_float(over_lanes(as_int(x), 0, [](int a, int b) {
+    return as_int(as_float(a) + as_float(b));
+  }));
+}
+
+// The lanes' sums as if one lane had seen all.
 __device__ __forceinline__ void join_lanes(Sums& a) {
-  const float m = ds::wave_reduce_max(a.m);
+  const float m = lanes_max(a.m);
   const float d2 = (a.m - m) * LOG2E, f = power(d2);
   float u = a.s > 0.f ? f * __builtin_fmaf(a.s, d2, a.u) : 0.f;
   float s = a.s * f;
   if (a.s != a.s) s = u = a.s;
-  a.s = ds::wave_reduce_sum(s);
-  a.u = ds::wave_reduce_sum(u);
+  a.s = lanes_sum(s);
+  a.u = lanes_sum(u);
   a.m = m;
 }
 __device__ __forceinline__ void join_waves(Sums& a, float (*lds)[3]) {
@@ -198,17 +231,15 @@ __device__ __forceinline__ float logit_of(unsigned key) {
 
 // The lane whose key is the largest, of equal ones the lowest id.
 __device__ __forceinline__ int best_lane(unsigned key, int id) {
-  unsigned top = key;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    top = max(top, (unsigned)__shfl_xor((int)top, off, 64));
-  unsigned long long who = __ballot(key == top);
+  const int top = over_lanes((int)key, 0, [](int a, int b) {
+    return (int)max((unsigned)a, (unsigned)b);
+  });
+  unsigned long long who = __ballot(key == (unsigned)top);
   if (who & (who - 1)) {
-    int low = key == top ? id : 0x7fffffff;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1)
-      low = min(low, __shfl_xor(low, off, 64));
-    who = __ballot(key == top && id == low);
+    const int low = over_lanes(key == (unsigned)top ? id : 0x7fffffff,
+                               0x7fffffff,
+                               [](int a, int b) { return min(a, b); });
+    who = __ballot(key == (unsigned)top && id == low);
   }
   return __builtin_ctzll(who);
 }
@@ -231,7 +262,7 @@ __global__ __launch_bounds__(CT) void parts_kernel(
   const int ahead = (int)(((uintptr_t)x & 15) / sizeof(T));
   const long long first = (long long)part * PART + tid * N - ahead;
   float v[HELD];
-  unsigned gone = 0;                   // places that are none, or were taken
+  unsigned gone = 0;                   // places that are none
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const long long j = first + (long long)c * CT * N;
@@ -262,28 +293,32 @@ __global__ __launch_bounds__(CT) void parts_kernel(
   }
   Best* list =
       lists + (((long long)row * parts + part) * (CT / 64) + wid) * top;
-  unsigned key = 0;
-  int place = 0;
+  if (top == 0) return;
+  unsigned keys[HELD], key = 0;
+#pragma unroll
+  for (int e = 0; e < HELD; ++e) keys[e] = gone >> e & 1 ? 0u : key_of(v[e]);
+  int place = -1;
+  // the lane's best but for `place`, which was taken
   auto look = [&]() __attribute__((always_inline)) {
+    const int taken = place;
     key = 0;
     place = 0;
 #pragma unroll
     for (int e = 0; e < HELD; ++e) {
-      const unsigned k = gone >> e & 1 ? 0u : key_of(v[e]);
-      if (k > key) {
-        key = k;
+      if (e == taken) keys[e] = 0;
+      if (keys[e] > key) {
+        key = keys[e];
         place = e;
       }
     }
   };
-  if (top) look();
+  look();
   for (int i = 0; i < top; ++i) {
     const int id =
         (int)(first + (long long)(place / N) * CT * N + place % N);
     const int who = best_lane(key, id);
     if (lane == who) {
       list[i] = Best{key, id};         // key 0: the wave has no more
-      gone |= 1u << place;
       look();
     }
   }

@@ -98,10 +98,15 @@ def paged_decode_attention(q: torch.Tensor, kpool: torch.Tensor,
     form of ``masked_attention``. There a block id that is not in the pool gives
     NaN for its request, and a length of 0 gives 0."""
     ext = get_ext()
-    scale = scale if scale is not None else 1.0 / math.sqrt(q.size(-1))
     if softcap or alibi_slopes is not None:
-        return _shaped(q, kpool, vpool, block_table, lens, splits, scale, softcap,
-                       alibi_slopes)
+        if splits is not None and splits < 1:
+            raise ValueError("paged_decode_attention: at least one split")
+        if q.is_cuda and ext is not None:
+            return ext.paged_shaped(q, kpool, vpool, block_table, lens, splits or 0,
+                                    scale, softcap, alibi_slopes)
+        return _torch_shaped(q, kpool, vpool, block_table, lens, scale, softcap,
+                             alibi_slopes)
+    scale = scale if scale is not None else 1.0 / math.sqrt(q.size(-1))
     if splits is None:
         nw = max(1, q.size(0) * kpool.size(1))
         splits = max(1, min(32, WORKGROUPS // nw))
@@ -110,8 +115,8 @@ def paged_decode_attention(q: torch.Tensor, kpool: torch.Tensor,
                             lens.contiguous().int(), splits, scale)
 
 
-def _shaped(q, kpool, vpool, block_table, lens, splits, scale, softcap, slopes):
-    """``paged_decode_attention`` of capped scores or with a bias by distance."""
+def _torch_shaped(q, kpool, vpool, block_table, lens, scale, softcap, slopes):
+    """The formulas over the gathered rows, in fp32 (fp64 for fp64)."""
     from .masked_attention import _checked_cap, _checked_slopes
     what = "paged_decode_attention"
     softcap = _checked_cap(softcap, what)
@@ -124,26 +129,9 @@ def _shaped(q, kpool, vpool, block_table, lens, splits, scale, softcap, slopes):
     if block_table.dim() != 2 or block_table.shape[0] != q.shape[0] or \
             lens.shape != q.shape[:1]:
         raise ValueError(f"{what}: block_table is [n, blocks], lens [n]")
-    if any(x.device != q.device for x in (kpool, vpool, block_table, lens)):
-        raise ValueError(f"{what}: tensors on different devices")
     slopes = _checked_slopes(slopes, q, what)
-    ext = get_ext()
-    if not q.is_cuda or ext is None:
-        return _torch_shaped(q, kpool, vpool, block_table, lens, scale, softcap,
-                             slopes)
-    if not paged_decode_available(q, kpool) or kpool.dtype is not torch.bfloat16 or \
-            vpool.dtype is not torch.bfloat16:
-        raise ValueError(f"{what}: bf16, heads of 128 and up to 16 a key head on a GPU")
-    if splits is None:
-        splits = max(1, min(32, WORKGROUPS // max(1, q.size(0) * kpool.size(1))))
-    return ext.paged_decode(aligned(q), aligned(kpool), aligned(vpool),
-                            block_table.contiguous().int(), lens.contiguous().int(),
-                            splits, scale, softcap, slopes)
-
-
-def _torch_shaped(q, kpool, vpool, block_table, lens, scale, softcap, slopes):
-    """The same formulas over the gathered rows, in fp32 (fp64 for fp64)."""
     n, H, D = q.shape
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
     blocks, Hkv, bs, _ = kpool.shape
     wide = torch.float64 if q.dtype is torch.float64 else torch.float32
     lens = lens.long().clamp(0, block_table.shape[1] * bs)

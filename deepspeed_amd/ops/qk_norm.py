@@ -57,7 +57,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
                                 layout == "half", one_plus)
     D = q.shape[-1] if q.dim() else 0
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or \
-            k.shape[3] != D or D % 2 or not 2 <= D <= 512:
+            k.shape[3] != D or D % 2 or not 2 <= D <= 512 or \
+            0 in (q.shape[2], k.shape[2]):
         raise ValueError("qk_norm_rope: q is [B, S, H, D], k [B, S, Hk, D], D even and "
                          f"up to 512, got {tuple(q.shape)} and {tuple(k.shape)}")
     if q_weight.shape != (D,) or k_weight.shape != (D,):
