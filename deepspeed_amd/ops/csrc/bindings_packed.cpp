@@ -287,6 +287,35 @@ Tensor aligned(const Tensor& t) {     // contiguous, on 16 bytes
   return (uintptr_t)x.data_ptr() % 16 == 0 ? x : x.clone();
 }
 
+// Parts of each request, of whose keys the table's width is all that the host knows. us
+// from cold caches, whole / in these parts, groups of heads times requests by keys:
+//   up to 512 keys whole: 8 x 350 8.7, in two parts 10.0
+//   up to 80 groups a workgroup a CU, of 125 keys at least: 8 x 700 13.0 / 10.8, 8 x
+//     4000 47 / 13, 32 x 4000 49 / 19, 72 x 12000 138 / 67
+//   more: whole up to 1024 keys (136 x 700 14.7, in 5 parts 16.7), and where they come
+//     to nearly one a CU (216 x 4000 58.8, in 7 parts 60.5; 256 x 2000 35.8, in 3 parts
+//     40.0), but for very long ones
+//   else the fewest parts, of 500 keys at least, that fill nine tenths of a round of
+//     three workgroups a CU: 136 x 4000 52 / 43, 288 x 4000 96 / 77, 384 x 4000 110 /
+//     99, 864 x 4000 200 / 187, 216 x 12000 157 / 140
+int64_t shaped_splits(int64_t groups, int64_t keys) {
+  if (keys <= 512) return 1;
+  if (groups <= 80) return std::clamp<int64_t>(256 / groups, 1,
+                                               std::clamp<int64_t>(keys / 125, 1, 32));
+  if (keys <= 1024 || (groups >= 176 && groups <= 256 && keys < 8000)) return 1;
+  const int64_t most = std::min<int64_t>(16, keys / 500);
+  int64_t best = 1;
+  double fill = 0;
+  for (int64_t n = 1; n <= most && fill < 0.9; ++n) {
+    const int64_t all = groups * n, rounds = (all + 767) / 768;
+    if (all / (768.0 * rounds) > fill && (all >= 700 || n == 1)) {
+      fill = all / (768.0 * rounds);
+      best = n;
+    }
+  }
+  return best;
+}
+
 // splits 0: by sizes.
 Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
                     const Tensor& vpool_, const Tensor& table_,
@@ -323,16 +352,7 @@ Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
   const int64_t BS = kpool.size(2), groups = n * Hkv;
   auto o = at::empty_like(q);
   if (n == 0) return o;
-  if (splits == 0) {
-    // One launch up to 1024 keys a request, which the table's width bounds (us, whole
-    // / cut for 1024 workgroups and merged: 1 x 700, 8 key heads 11.5 / 13.8; 32 x 700
-    // 14.2 / 19.7). Longer ones in parts of 500 keys and more: few requests for a
-    // workgroup a CU (9 x 4000 25.4 / 26.2, 9 x 12000 60.5 / 70.6), many for up to
-    // twelve (48 x 4000 87 / 92, 40 x 4000 71 / 73, 136 groups of 12000 97 / 104).
-    const int64_t keys = table.size(1) * BS;
-    splits = keys <= 1024 ? 1 : 2 * groups <= 256 ? 256 / groups : 3072 / groups;
-    splits = std::max<int64_t>(1, std::min({splits, keys / 500, (int64_t)32}));
-  }
+  if (splits == 0) splits = shaped_splits(groups, table.size(1) * BS);
   TORCH_CHECK_VALUE(splits >= 1 && kpool.size(0) > 0 &&
                     kpool.size(0) < (1ll << 31) && H * 128 < (1ll << 31) &&
                     n * splits * 512 < THREADS && Hkv <= 65535 &&

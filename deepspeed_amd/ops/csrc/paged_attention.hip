@@ -59,7 +59,7 @@ using attn::mfma;
 
 constexpr int D = 128;
 constexpr int KT = 32;        // keys a tile
-constexpr int attn_waves = 4; // waves a workgroup
+constexpr int NW = 4;         // waves a workgroup
 constexpr int OSTR = D + 4;   // floats between columns of a merged tile
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -166,9 +166,8 @@ struct Keys {
 // SHAPED: the scores are capped, fall with the distance, or both (no runs). They leave
 // the first product for units of log2 at once and the rest goes on with c = 1. A block
 // of the table that is not in the pool makes its request's row NaN.
-template <int NQ, bool ALIGNED, bool SHAPED, int NW = attn_waves>
-__global__ __launch_bounds__(NW * 64, NW > 4 || NQ > 1 ? 2 : 3) void rows_kernel(
-    const Args a) {
+template <int NQ, bool ALIGNED, bool SHAPED>
+__global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) float lds[NW][16 * OSTR];
   __shared__ float lds_ml[NW][NQ * 16][2];
   static_assert(16 * OSTR * 4 >= KT * D * 2, "the V tile fits");
@@ -384,7 +383,7 @@ __global__ __launch_bounds__(NW * 64, NW > 4 || NQ > 1 ? 2 : 3) void rows_kernel
     __syncthreads();
     const int c = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
     const int rr = (tile * NQ + n) * 16 + c;
-    if (rr < ncols && (NW <= 4 || c < 16)) {
+    if (rr < ncols) {
       float mg = -1e30f, lg = 0.f, o[8] = {};
 #pragma unroll
       for (int w = 0; w < NW; ++w) mg = fmaxf(mg, lds_ml[w][n * 16 + c][0]);
@@ -856,10 +855,10 @@ int launch_rows(const Args& a, const int2* merges, int n_items, int n_merges,
                           : launch_block<false>(a, n_items, st);
     if (e) return e;
   } else if (aligned) {
-    hipLaunchKernelGGL((rows_kernel<NQ, true, false>), grid, dim3(attn_waves * 64), 0,
+    hipLaunchKernelGGL((rows_kernel<NQ, true, false>), grid, dim3(NW * 64), 0,
                        st, a);
   } else {
-    hipLaunchKernelGGL((rows_kernel<NQ, false, false>), grid, dim3(attn_waves * 64), 0,
+    hipLaunchKernelGGL((rows_kernel<NQ, false, false>), grid, dim3(NW * 64), 0,
                        st, a);
   }
   if (any_merge)
@@ -952,16 +951,12 @@ extern "C" int ds_paged_shaped(const void* q, const void* kpool,
   a.blocks = blocks;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(n * splits, Hkv);
-  const bool whole = BS % KT == 0;
-  if (splits == 1 && n * Hkv <= 256) {
-    const auto kernel = whole ? rows_kernel<1, true, true, 8>
-                              : rows_kernel<1, false, true, 8>;
-    hipLaunchKernelGGL(kernel, grid, dim3(512), 0, st, a);
-  } else {
-    const auto kernel =
-        whole ? rows_kernel<1, true, true> : rows_kernel<1, false, true>;
-    hipLaunchKernelGGL(kernel, grid, dim3(attn_waves * 64), 0, st, a);
-  }
+  if (BS % KT == 0)
+    hipLaunchKernelGGL((rows_kernel<1, true, true>), grid, dim3(NW * 64), 0, st,
+                       a);
+  else
+    hipLaunchKernelGGL((rows_kernel<1, false, true>), grid, dim3(NW * 64), 0,
+                       st, a);
   if (splits > 1)
     hipLaunchKernelGGL((merge_kernel<1>), dim3(n, Hkv, 4), dim3(128), 0, st, a,
                        (const int2*)nullptr);
