@@ -84,14 +84,26 @@ __device__ __forceinline__ s16x8 operand(const f32x16& p, int s) {
 
 // Tile of rows of D bf16 in LDS. Within a row the swizzle is an exclusive or,
 // so the addresses of one lane's reads differ by one from a first one.
-template <int D>
+//
+// FANNED: the four rows of a transposing read lie in four different quarters of the
+// banks as well, whether 16 or 32 lanes are read at once, and the rows of 8 or 16 lanes
+// of a row-wise read in all of them. With a row's lower bits for its turn two and more
+// of the four rows share their banks: the LDS was busy for 72 to 82% of the time of the
+// masked attention's kernels, a third of that conflicts.
+template <int D, bool FANNED = false>
 struct Tile {
   static constexpr int CH = D / 8;                  // chunks of a row
   static constexpr int SC = D == 64 ? 8 : 16;       // places of a row
   static constexpr int RB = SC * 16;                // bytes of a row
   static __device__ __forceinline__ int turn(int row) {
-    return D == 64 ? (row >> 1) & 7 : row & 15;
+    if (!FANNED) return D == 64 ? (row >> 1) & 7 : row & 15;
+    const int b0 = row & 1, b1 = row >> 1 & 1, b2 = row >> 2 & 1,
+              b3 = row >> 3 & 1;
+    return D == 64 ? b2 | (b0 ^ b3) << 1 | b1 << 2
+                   : b2 | b1 << 1 | b0 << 2 | (b1 ^ b3) << 3;
   }
+  // what the turn of a row 8 further on differs by, in bytes
+  static constexpr int EIGHT = FANNED && D == 64 ? 32 : RB / 2;
   // A operand: rows row0 + col, contracted k = 16 kk + 8 half + j
   static __device__ __forceinline__ int rows_at(int lane) {
     const int col = lane & 31;
@@ -112,7 +124,7 @@ struct Tile {
   static __device__ __forceinline__ s16x8 cols(const short* t, int row0,
                                                int db, int at) {
     const char* p = (const char*)t + row0 * RB;
-    const int lo = at ^ (db * 64), hi = lo ^ (RB / 2);   // row + 8
+    const int lo = at ^ (db * 64), hi = lo ^ EIGHT;       // row + 8
     const s16x4 a = tr_read((const short*)(p + lo));
     const s16x4 b = tr_read((const short*)(p + 8 * RB + hi));
     return s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(const Ar
                                                          const int heads) {
   constexpr int KT = KB / 32, DB = D / 32, KK = D / 16, QB = 32 * NW, TPB = 64 * NW;
   constexpr bool PLAIN = !CAP && !BIAS;
-  using T = Tile<D>;
+  using T = Tile<D, true>;
   __shared__ __attribute__((aligned(16))) short kt[2][KB * T::SC * 8];
   __shared__ __attribute__((aligned(16))) short vt[2][KB * T::SC * 8];
 
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
                                                       const int heads) {
   constexpr int QB = 64, DB = D / 32, KK = D / 16;
   constexpr bool PLAIN = !CAP && !BIAS;
-  using T = Tile<D>;
+  using T = Tile<D, true>;
   __shared__ __attribute__((aligned(16))) short qt[2][QB * T::SC * 8];
   __shared__ __attribute__((aligned(16))) short dt[2][QB * T::SC * 8];
   __shared__ __attribute__((aligned(16))) float st[2][2][QB];
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
                                                     const int heads) {
   constexpr int KB = 64, DB = D / 32, KK = D / 16;
   constexpr bool PLAIN = !CAP && !BIAS;
-  using T = Tile<D>;
+  using T = Tile<D, true>;
   __shared__ __attribute__((aligned(16))) short kt[2][KB * T::SC * 8];
   __shared__ __attribute__((aligned(16))) short vt[2][KB * T::SC * 8];
 
