@@ -573,9 +573,9 @@ variable_list logprobs_fwd(const Tensor& x, const Tensor& tokens, int64_t top,
   best.push_back(top);
   auto top_lp = at::empty(best, f32), ids = at::empty(best, tokens.options());
   if (r.rows) {
-    // the parts' sums, then on 8 bytes the waves' lists
+    // the parts' sums, then on 8 bytes their lists
     const int64_t of_sums = (r.rows * parts * 3 + 1) / 2 * 2;
-    auto work = at::empty({of_sums + r.rows * parts * 8 * top}, f32);
+    auto work = at::empty({of_sums + r.rows * parts * 2 * top}, f32);
     float* sums = work.data_ptr<float>();
     const int e = ds_logprobs_fwd(
         x.data_ptr(), r.outer_stride, r.inner_stride, (int)r.inner, r.type,

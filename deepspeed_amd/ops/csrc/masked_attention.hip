@@ -701,14 +701,12 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
       const int key0 = k0 + 32 * t;
       if (key0 >= any1 || key0 + 32 <= any0) continue;
       f32x16 p = {}, dp = {};
-      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
         p = mfma(T::rows(kt[cur], 32 * t, kk, ra), qf[kk], p);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
         dp = mfma(T::rows(vt[cur], 32 * t, kk, ra), df[kk], dp);
-      __builtin_amdgcn_s_setprio(0);
       const float far = (float)(key0 + 4 * half - at);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -728,7 +726,6 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
           if ((unsigned)((r & 3) + 8 * (r >> 2) - first) >= (unsigned)width)
             dp[r] = 0.f;
       }
-      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const s16x8 sb = operand(dp, s);
@@ -737,7 +734,6 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
           acc[db] =
               mfma(T::cols(kt[cur], 32 * t + 16 * s, db, ca), sb, acc[db]);
       }
-      __builtin_amdgcn_s_setprio(0);
     }
     arrive();
   }
