@@ -114,7 +114,6 @@ struct MaskedArgs : FlashArgs {
   MaskedArgs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
              const Opt& spans_, const Opt& slopes_, double scale, double cap)
       : FlashArgs(q, k, v, scale) {
-    TORCH_CHECK(cap >= 0 && cap < 1e30, "masked_attention: softcap");
     TORCH_CHECK((int64_t)B * H * ((S + 127) / 128) * 256 < THREADS,
                 "masked_attention: size");
     if (data(spans_)) {
@@ -248,7 +247,7 @@ Opt slopes_of(const Opt& t, const Tensor& q, const char* what) {
 }
 
 void check_cap(double softcap, const char* what) {
-  TORCH_CHECK_VALUE(softcap >= 0 && softcap < 1e30, what,
+  TORCH_CHECK_VALUE(softcap == 0 || (softcap > 1e-30 && softcap < 1e30), what,
                     ": softcap is 0 (none) or positive, got ", softcap);
 }
 
@@ -258,7 +257,8 @@ Tensor masked_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   TORCH_CHECK_VALUE(
       q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() &&
       q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
-      q.size(3) == k.size(3) && k.size(2) > 0 && q.size(2) % k.size(2) == 0,
+      q.size(3) == k.size(3) && k.size(2) > 0 && q.size(2) > 0 &&
+      q.size(2) % k.size(2) == 0,
       "masked_attention: q is [B, S, H, D], k and v are [B, S, Hkv, D] with H a "
       "multiple of Hkv, got ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
   TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type() &&
@@ -620,7 +620,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
                                int64_t ignore) {
     // up to three dimensions of any strides but one inside a row
     auto x = logits;
-    if (x.dim() > 3) x = x.reshape({-1, x.size(-2), x.size(-1)});
+    if (x.dim() > 3) x = x.flatten(0, x.dim() - 3);
     if (x.size(-1) > 1 && x.stride(-1) != 1) x = x.contiguous();
     auto out = logprobs_fwd(x, tokens, top, ignore);
     ctx->save_for_backward({x, tokens, out[2], out[1]});

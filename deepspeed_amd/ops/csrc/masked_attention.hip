@@ -16,9 +16,10 @@
 // attention.hip, which says why.
 //
 // The matrix cores add 0 times what a hidden row holds, which is no 0 for an
-// infinity or NaN there: a row whose sums are not finite though its own statistics
-// are is summed again over what it sees alone (the loops over `bad` below, which
-// nothing reaches with finite inputs).
+// infinity or NaN there: a row whose sums are not finite though all that it sees is,
+// by its statistics or by a look, is summed again over that alone (the loops over
+// `bad` below, which nothing reaches with finite inputs, and of the rest only rows that
+// share a tile with something hidden that is not finite).
 
 #include "attention_tile.h"
 #include "ds_kernels.h"
@@ -47,6 +48,7 @@ struct Args {
   int B, S, H, Hkv, causal;
   float scale, c;         // c: scale * log2(e)
   float a, cap;           // a: 2 log2(e) scale / cap, cap: cap * log2(e)
+  float x;                // scale / cap
 };
 
 struct Span {
@@ -98,7 +100,11 @@ __device__ __forceinline__ float add_pairs(s16x8 x, float t) {
 // where all of a tile's scores are near 0 takes two thirds of its instructions and was
 // 4% less of the forward and nothing of the rest: the matrix cores' operands, not
 // these, are what a step waits for.)
-template <bool CAP, bool BIAS>
+// That 1 - 2 / (..) is off by 2^-23 of the cap, wherever x is: nothing beside bf16 for
+// caps up to 200. WIDE ones take the series of tanh up to x of 1/4, to 3e-7 of itself.
+enum Cap { NONE, USUAL, WIDE };
+
+template <int CAP, bool BIAS>
 struct Score {
   const Args& a;
   const float slope;
@@ -110,6 +116,13 @@ struct Score {
           __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.a) + 1.f);
       t = __builtin_fmaf(-2.f * a.cap, r, a.cap);
       bend = 4.f * r * (1.f - r);
+      if (CAP == WIDE) {
+        const float x = s * a.x, y = x * x;
+        float p = __builtin_fmaf(y, -17.f / 315, 2.f / 15);
+        p = __builtin_fmaf(y, p, -1.f / 3);
+        p = __builtin_fmaf(y, p, 1.f);
+        if (__builtin_fabsf(x) < 0.25f) t = s * a.c * p;
+      }
     } else {
       t = s * a.c;
     }
@@ -166,7 +179,7 @@ __device__ __forceinline__ void settle(s16x8 (&x)[N]) {
 
 // ------------------------------------------------------------------ forward
 
-template <int D, bool CAP, bool BIAS, int NW, int KB>
+template <int D, int CAP, bool BIAS, int NW, int KB>
 __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(const Args a,
                                                          const int blocks,
                                                          const int heads) {
@@ -339,7 +352,29 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(const Ar
   }
   unsigned long long bad = __ballot(real && !good && finite(sum));
   bad = (bad | bad >> 32) & 0xffffffffull;
-  if (bad) __builtin_amdgcn_s_waitcnt(0);      // the rows as they were written
+  if (bad) {
+    // the first and the last of the wave's keys whose value is not finite: a row that
+    // sees one of them is as it is
+    int low = S, high = -1;
+    for (int j = any0 + lane; j < any1; j += 64) {
+      const short* vj = vp + j * a.vv.s;
+      bool sick = false;
+      for (int d = 0; d < D; ++d) sick = sick || !finite(value(vj[d]));
+      if (sick) {
+        low = min(low, j);
+        high = j;
+      }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      low = min(low, __shfl_xor(low, off, 64));
+      high = max(high, __shfl_xor(high, off, 64));
+    }
+    const bool sees = (low >= me.lo && low < me.hi) ||
+                      (high >= me.lo && high < me.hi);
+    bad &= ~__ballot(sees);
+    __builtin_amdgcn_s_waitcnt(0);      // the rows as they were written
+  }
   for (; bad; bad &= bad - 1) {
     const int n = __builtin_ctzll(bad), i = q0 + n;
     const int lo = lane_of(me.lo, n), hi = lane_of(me.hi, n);
@@ -371,7 +406,7 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(const Ar
 // ----------------------------------------------------------------- backward
 
 // dK and dV: a wave owns 32 keys and walks the queries that see them.
-template <int D, bool CAP, bool BIAS>
+template <int D, int CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
                                                       const int blocks,
                                                       const int heads) {
@@ -553,6 +588,13 @@ __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
   for (; bad; bad &= bad - 1) {
     const int w = __builtin_ctzll(bad), j = k0 + w;
     const int lo = lane_of(me.lo, w), hi = lane_of(me.hi, w);
+    bool sick = false;      // a row that sees the key
+    for (int head = hkv * G + g0; head < hkv * G + g1; ++head)
+      for (int i = lo + lane; i < hi; i += 64) {
+        const long long u = ((long long)b * a.H + head) * S + i;
+        sick = sick || !finite(a.lse[u]) || !finite(a.stat[u]);
+      }
+    if (__any(sick)) continue;
     const short* kj = a.k + b * a.vk.b + hkv * a.vk.h + j * a.vk.s;
     const short* vj = a.v + b * a.vv.b + hkv * a.vv.h + j * a.vv.s;
     float k_0 = 0.f, k_1 = 0.f, v_0 = 0.f, v_1 = 0.f;
@@ -619,7 +661,7 @@ __global__ __launch_bounds__(256) void add_kernel(
 }
 
 // dQ: a wave owns 32 queries and walks the keys that they see.
-template <int D, bool CAP, bool BIAS>
+template <int D, int CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
                                                     const int blocks,
                                                     const int heads) {
@@ -870,7 +912,7 @@ __global__ __launch_bounds__(ST) void spans_kernel(
   y[3 * n] = e;
 }
 
-template <int D, bool CAP, bool BIAS, int NW, int KB>
+template <int D, int CAP, bool BIAS, int NW, int KB>
 int launch_fwd(const Args& a, hipStream_t s) {
   const int blocks = (a.S + 32 * NW - 1) / (32 * NW), heads = a.B * a.H;
   hipLaunchKernelGGL((fwd_kernel<D, CAP, BIAS, NW, KB>),
@@ -879,7 +921,7 @@ int launch_fwd(const Args& a, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int CAP, bool BIAS>
 int launch_bwd(const Args& a, int splits, hipStream_t s) {
   const int blocks = (a.S + 127) / 128;
   hipLaunchKernelGGL((dq_kernel<D, CAP, BIAS>),
@@ -898,7 +940,7 @@ int launch_bwd(const Args& a, int splits, hipStream_t s) {
 
 template <int D>
 int launch(const Args& a, int splits, hipStream_t s) {
-  const bool cap = a.cap > 0.f, bias = a.slopes != nullptr;
+  const bool bias = a.slopes != nullptr;
   // Steps of 32 keys leave room for three workgroups a CU where heads of 96 and 128
   // need registers for two otherwise (us, 64 / 32 keys: 1 x 8192 capped 811 / 769, nine
   // documents in 4 x 4096 258 / 230, heads of 96 273 / 250); heads of 64 hold four
@@ -907,8 +949,9 @@ int launch(const Args& a, int splits, hipStream_t s) {
 #define GO(C, W)                      \
   (splits ? launch_bwd<D, C, W>(a, splits, s) \
           : launch_fwd<D, C, W, 4, KB>(a, s))
-  if (cap) return bias ? GO(true, true) : GO(true, false);
-  return bias ? GO(false, true) : GO(false, false);
+  if (a.cap == 0.f) return bias ? GO(NONE, true) : GO(NONE, false);
+  if (a.cap <= 200.f * LOG2E) return bias ? GO(USUAL, true) : GO(USUAL, false);
+  return bias ? GO(WIDE, true) : GO(WIDE, false);
 #undef GO
 }
 
@@ -953,7 +996,8 @@ extern "C" int ds_masked_attention(
   a.scale = scale;
   a.c = scale * LOG2E;
   a.cap = cap * LOG2E;
-  a.a = cap > 0.f ? 2.f * LOG2E * scale / cap : 0.f;
+  a.x = cap > 0.f ? scale / cap : 0.f;
+  a.a = 2.f * LOG2E * a.x;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (D == 64) return launch<64>(a, splits, s);
   if (D == 96) return launch<96>(a, splits, s);

@@ -84,7 +84,8 @@ struct Args {
   // log2, and no block of the table outside of the pool's
   const float* slopes;  // [H] or null
   float a2, cap;        // 2 log2(e) scale / cap, cap * log2(e), or 0 and 0
-  float sc;             // scale * log2(e)
+  float sc, x;          // scale * log2(e), scale / cap
+  bool wide;            // a cap over 200: as masked_attention.hip
   int blocks;
 };
 
@@ -305,6 +306,13 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
                   __builtin_amdgcn_rcpf(
                       __builtin_amdgcn_exp2f(s[n][t][r] * a.a2) + 1.f),
                   a.cap);
+            if (a.wide) {
+              const float z = s[n][t][r] * a.x, zz = z * z;
+              float p = __builtin_fmaf(zz, -17.f / 315, 2.f / 15);
+              p = __builtin_fmaf(zz, p, -1.f / 3);
+              p = __builtin_fmaf(zz, p, 1.f);
+              if (__builtin_fabsf(z) < 0.25f) y = s[n][t][r] * a.sc * p;
+            }
             s[n][t][r] = __builtin_fmaf(-slope[n], far - (16 * t + r), y);
           }
       }
@@ -912,7 +920,8 @@ extern "C" int ds_paged_rows(const void* q, const void* kpool,
   a.c = fabsf(scale) * LOG2E;
   a.flip = scale < 0.f;
   a.slopes = nullptr;
-  a.a2 = a.cap = a.sc = 0.f;
+  a.a2 = a.cap = a.sc = a.x = 0.f;
+  a.wide = false;
   a.blocks = 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int2* mg = (const int2*)merges;
@@ -947,7 +956,9 @@ extern "C" int ds_paged_shaped(const void* q, const void* kpool,
   a.slopes = slopes;
   a.sc = scale * LOG2E;
   a.cap = cap * LOG2E;
-  a.a2 = cap > 0.f ? 2.f * LOG2E * scale / cap : 0.f;
+  a.x = cap > 0.f ? scale / cap : 0.f;
+  a.a2 = 2.f * LOG2E * a.x;
+  a.wide = cap > 200.f;
   a.blocks = blocks;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(n * splits, Hkv);

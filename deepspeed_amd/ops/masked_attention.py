@@ -118,7 +118,7 @@ def _checked_slopes(alibi_slopes, q, what):
 
 def _checked_cap(softcap, what):
     softcap = float(softcap or 0.0)
-    if not 0.0 <= softcap < 1e30:
+    if softcap != 0.0 and not 1e-30 < softcap < 1e30:
         raise ValueError(f"{what}: softcap is 0 (none) or positive, got {softcap}")
     return softcap
 
@@ -140,7 +140,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                     softcap or 0.0)
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or \
             q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or \
-            k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+            0 in (q.shape[2], k.shape[2]) or q.shape[2] % k.shape[2]:
         raise ValueError("masked_attention: q is [B, S, H, D], k and v are [B, S, Hkv, "
                          "D] with H a multiple of Hkv, got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")

@@ -18,7 +18,7 @@ def _torch_heads(x, weight, cos, sin, positions, eps, layout, one_plus):
     B, S, _, D = x.shape
     n = 2 * cos.shape[1]
     at = torch.arange(S, device=x.device).expand(B, S) if positions is None \
-        else positions.view(B, S).long()
+        else positions.reshape(B, S).long()
     there = (at >= 0) & (at < cos.shape[0])
     c, s = (torch.where(there[..., None], t[torch.where(there, at, 0)], float("nan"))
             .to(wide)[:, :, None] for t in (cos, sin))

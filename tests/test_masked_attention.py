@@ -91,6 +91,11 @@ def _reference(q, k, v, do, seen, scale, cap, slopes):
     off_ds = BF16 * ds.abs() + bend * p * (
         off_delta + FP32 * (dp.abs() + delta.abs()
                             + do.abs() @ vt.abs()))
+    if cap:
+        # 1 - tanh^2 = 4 r (1 - r) of an r = 1 / (e^2x + 1) up to 1 in fp32: r is off by
+        # 2^-23 (its sum and its reciprocal by 2^-24 each), 1 - r is exact from 1/2 on,
+        # so four times their product by up to 4 x 2^-23, be it ever so small
+        off_ds = off_ds + 2.0 ** -21 * p * (dp.abs() + delta.abs())
     off_ds = torch.where(seen, off_ds, 0.0)
     off = [off_o, off_ds @ k.abs() * abs(scale),
            group(off_ds.transpose(2, 3).contiguous() @ q.abs()) * abs(scale),
@@ -584,3 +589,74 @@ def test_second_derivatives_raise_gpu():
     assert torch.equal(dv, plain[2])
     with torch.no_grad():
         assert not masked_attention(*leaves).requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 200.0, 201.0, 1e3, 1e5, 1e20])
+def test_caps_gpu(cap):
+    """Caps far below and far above the scores: what is left of them is as exact."""
+    ids = _ids([[90, 40]])
+    seen = _seen(ids, None, True).cuda()
+    q, k, v, do = _inputs(1, 130, 4, 2, 64, "cuda", seed=13, spread=4)
+    got = _grads(q, k, v, do, packed_rows(ids.cuda()), softcap=cap)
+    _check(got, *_reference(q, k, v, do, seen, 0.125, cap, None))
+    q, kp, vp, table, n = _decode_inputs([130, 75], 8, 2, 16, "cuda", spread=4)
+    o = paged_decode_attention(q, kp, vp, table, n, softcap=cap)
+    want, off = _decode_reference(q, kp, vp, table, n, 128 ** -0.5, cap, None)
+    assert ((o.double().cpu() - want).abs() <= off).all()
+
+
+@pytest.mark.gpu
+def test_far_rows_gpu():
+    """Rows and blocks whose places do not fit 32 bits."""
+    far = torch.empty(1, 300, 1 << 23, dtype=torch.bfloat16, device="cuda")
+    q, k, v, do = _inputs(1, 300, 2, 1, 128, "cuda", seed=15)
+    want = _grads(q, k, v, do, None, softcap=20.0)
+    there = []
+    for i, x in enumerate((q, k, v, do)):
+        y = far[:, :, i * 4096:i * 4096 + x.shape[2] * 128].unflatten(-1, (-1, 128))
+        there.append(y.copy_(x))
+    got = _grads(*there, None, softcap=20.0)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    del far, there, got
+    q, kp, vp, table, n = _decode_inputs([130, 75], 8, 2, 64, "cuda")
+    want = paged_decode_attention(q, kp, vp, table, n, softcap=20.0)
+    first = (1 << 31) // (2 * 64 * 128) + 1
+    pools = [torch.empty(first + len(kp), 2, 64, 128, dtype=torch.bfloat16,
+                         device="cuda") for _ in "kv"]
+    for pool, x in zip(pools, (kp, vp)):
+        pool[first:] = x
+    table = torch.where(table < 0, table, table + first)
+    assert torch.equal(want, paged_decode_attention(q, *pools, table, n, softcap=20.0))
+
+
+@pytest.mark.gpu
+def test_seen_infinities_gpu():
+    """What a query does see stays what it is: rows behind a value that is not finite,
+    gradients that are not, and the rows and keys apart from them."""
+    q, k, v, do = _inputs(1, 300, 2, 1, 64, "cuda", seed=17)
+    ids = _ids([[200, 100]])
+    rows = packed_rows(ids.cuda())
+    want = _reference(q, k, v, do, _seen(ids, None, True).cuda(), 0.125, 0.0, None)
+
+    def near(name, x, part):
+        i = ("o", "dq", "dk", "dv").index(name)
+        assert ((x.double() - want[0][i]).abs() <= want[1][i])[0, part].all(), name
+
+    sick = v.clone()
+    sick[0, 40] = float("inf")
+    got = _grads(q, k, sick, do, rows)
+    assert (got[0][0, 40:200] == float("inf")).all()
+    near("o", got[0], slice(200, None))
+    near("o", got[0], slice(40))
+    for name, x in zip(("dq", "dk", "dv"), got[1:]):
+        near(name, x, slice(200, None))
+    near("dq", got[1], slice(40))
+    do = do.clone()
+    do[0, 250] = float("nan")
+    got = _grads(q, k, v, do, rows)
+    for name, x in zip(("dq", "dk", "dv"), got[1:]):
+        near(name, x, slice(200))
+        near(name, x, slice(251, None))
+    near("dq", got[1], slice(250))
+    assert got[1][0, 250].isnan().all() and got[2][0, 200:251].isnan().all()

@@ -241,3 +241,17 @@ def test_graph_and_one_gradient_gpu():
     assert all(torch.equal(x, y) for x, y in zip(grads, want))
     empty = torch.empty(0, 3, 2, 64, dtype=torch.bfloat16, device="cuda")
     assert qk_norm_rope(empty, empty, *ins[2:6])[0].shape == empty.shape
+
+
+@pytest.mark.gpu
+def test_far_rows_gpu():
+    """Rows whose places do not fit 32 bits."""
+    far = torch.empty(1, 300, 1 << 23, dtype=torch.bfloat16, device="cuda")
+    ins, dy = _inputs(1, 300, 4, 2, 128, 128, torch.bfloat16, "cuda", table=300)
+    want = _run(ins, dy)
+    there = []
+    for i, x in enumerate((*ins[:2], *dy)):
+        y = far[:, :, i * 4096:i * 4096 + x.shape[2] * 128].unflatten(-1, (-1, 128))
+        there.append(y.copy_(x))
+    got = _run((*there[:2], *ins[2:]), there[2:])
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

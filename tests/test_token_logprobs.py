@@ -276,3 +276,31 @@ def test_nothing_and_refusals_gpu():
         token_logprobs(x.double(), y)
     with pytest.raises(ValueError, match="device"):
         token_logprobs(x, y.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("top", [0, 4])
+def test_far_rows_gpu(top):
+    """Rows whose places do not fit 32 bits, of the logits and of their gradient."""
+    far = torch.empty(600, 1 << 23, dtype=torch.bfloat16, device="cuda")
+    x, y, glp, gent = _inputs(600, 9001, torch.bfloat16, "cuda")
+    there = far[:, :9001].copy_(x)
+    _check(there, y, glp, gent, top)
+
+
+@pytest.mark.gpu
+def test_wide_gradient_gpu():
+    """A gradient of more than 2^31 numbers: its last rows."""
+    x = torch.zeros(17000, 128256, dtype=torch.bfloat16, device="cuda")
+    y = torch.full((17000,), IGNORE, device="cuda")
+    small, t, glp, gent = _inputs(5, 128256, torch.bfloat16, "cuda", ignored=0)
+    x[-5:], y[-5:] = small, t
+    leaf = x.requires_grad_()
+    got = token_logprobs(leaf, y)
+    dx, = torch.autograd.grad((got.logprobs[-5:], got.entropy[-5:]), leaf, (glp, gent))
+    want, dsmall = _check(small, t, glp, gent)
+    assert not dx[:-5].any()
+    # by whole rows here, by parts there: sums in other orders, roundings a step apart
+    torch.testing.assert_close(dx[-5:].float(), dsmall.float(), rtol=2.0 ** -7,
+                               atol=1e-7)
+    torch.testing.assert_close(got.logprobs[-5:], want.logprobs, rtol=1e-6, atol=1e-5)
