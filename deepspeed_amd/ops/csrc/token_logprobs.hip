@@ -9,7 +9,9 @@
 // fp32, of differences to the maximum, so that large logits cost no digits; x - m is
 // taken before it is scaled to a power of two for the same reason.
 //
-// Bound by the logits' stream: read once forward, read and written once backward.
+// Bound by the logits' stream, read once forward, read and written once backward, past
+// the caches, which they do not fit. 4096 x 128256 bf16: 146 us forward (7.2 TB/s; 199
+// through the caches), 405 backward (5.2 TB/s, a copy's rate).
 
 #include "ds_kernels.h"
 
@@ -81,7 +83,7 @@ struct Sums {
 
 // Over the 64 lanes by moves inside the vector unit: rows of 16, the rows of a half,
 // the halves; the last lane has it all. Six exchanges through LDS take as long as
-// thirty of these, and a best token takes one or two such reductions.
+// thirty of these.
 template <typename Op>
 __device__ __forceinline__ int over_lanes(int x, int none, Op op) {
 #define STEP(CTRL, ROWS) \
@@ -105,6 +107,11 @@ __device__ __forceinline__ float lanes_max(float x) {
   return as_float(over_lanes(as_int(x), as_int(LOWEST), [](int a, int b) {
     return as_int(fmaxf(as_float(a), as_float(b)));
   }));
+}
+__device__ __forceinline__ unsigned lanes_max(unsigned x) {
+  return over_lanes((int)x, 0, [](int a, int b) {
+    return (int)max((unsigned)a, (unsigned)b);
+  });
 }
 __device__ __forceinline__ float lanes_sum(float x) {
   return as_float(over_lanes(as_int(x), 0, [](int a, int b) {
@@ -229,7 +236,10 @@ __global__ __launch_bounds__(CT) void rows_kernel(
 // The best `top` of many, by lanes: the top-th largest of the lanes' own best is a
 // bound that `top` logits reach, and what reaches it, few more than those, is
 // gathered and put in its place by counting what is better. Taking one best after
-// another cost 1.7 us each (24 x 128256, 20 best: 37 us for 13).
+// another cost 1.2 us each (24 x 128256 in all, us, 5 best 16.5 and now 15.2, 20 best 37
+// and 20, 32 best 51 and 26); a single one is a maximum (128 rows 26.2 and 19.6).
+// Bound by latency: the parts' kernel
+// takes 4.7 us without best tokens, 10.5 with five, joining them 2.6 and 5.0.
 
 // A logit and its id as one number: larger logits first, of equal ones the lower id.
 // NaN lies above all, -0 is 0, and 0 stands for none.
@@ -356,17 +366,24 @@ __global__ __launch_bounds__(CT) void parts_kernel(
     }
   }
   const Rated mine = key ? rated(key, (int)first + at(place)) : 0;
-  const Rated low = bound(mine, better(mine, 64), top);
-  const unsigned low_key = (unsigned)(low >> 32);
-  int n = 0;
+  if (top == 1) {
+    const unsigned hi = lanes_max(key);
+    const unsigned lo = lanes_max(key == hi ? (unsigned)mine : 0u);
+    __syncthreads();
+    if (lane == 0) best[wid] = (Rated)hi << 32 | lo;
+  } else {
+    const Rated low = bound(mine, better(mine, 64), top);
+    const unsigned low_key = (unsigned)(low >> 32);
+    int n = 0;
 #pragma unroll
-  for (int e = 0; e < HELD; ++e)
-    if (__any(keys[e] >= low_key)) {
-      const Rated r = rated(keys[e], (int)first + at(e));
-      n = gather(held, n, r, keys[e] != 0 && r >= low);
-    }
-  __syncthreads();
-  places(held, n, top, [&](int r, Rated y) { best[wid * top + r] = y; });
+    for (int e = 0; e < HELD; ++e)
+      if (__any(keys[e] >= low_key)) {
+        const Rated r = rated(keys[e], (int)first + at(e));
+        n = gather(held, n, r, keys[e] != 0 && r >= low);
+      }
+    __syncthreads();
+    places(held, n, top, [&](int r, Rated y) { best[wid * top + r] = y; });
+  }
   __syncthreads();
   // the waves' lists into one: a place in one's own, and in each of the others
   if (tid < NW * top && best[tid] != 0) {
@@ -506,10 +523,13 @@ __global__ __launch_bounds__(CT) void grad_kernel(
 
 }  // namespace
 
-// Parts a row is cut into; 0: a workgroup a row.
+// Parts a row is cut into; 0: a workgroup a row, which saves a launch and the sums' way
+// through memory. us, whole rows and parts, bf16: 16 x 32000 9.1 and 11.7, 384 x 32000
+// 13.0 and 12.4, 16 x 128256 17.6 and 10.4, 128 26.3 and 15.5, 384 31.2 and 30.4,
+// 512 32.0 and 37.9, 2048 85.7 and 134.5.
 extern "C" int ds_logprobs_parts(int rows, long long V, int top) {
   const long long parts = (V + PART + 6) / PART;   // a row may begin inside a chunk
-  return top == 0 && (parts == 1 || rows >= 512) ? 0 : (int)parts;
+  return top == 0 && (parts <= 4 || rows >= 400) ? 0 : (int)parts;
 }
 
 // type: 0 fp32, 1 bf16, 2 fp16. parts as ds_logprobs_parts says, sums [N, parts, 3],
@@ -552,7 +572,9 @@ extern "C" int ds_logprobs_bwd(const void* x, long long outer_stride,
                                long long V, long long ignore, void* stream) {
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const Rows r = {x, outer_stride, inner_stride, inner};
-  // whole rows from 2048 on; fewer are cut, but not below 4096 logits
+  // whole rows from 2048 on; fewer are cut, but not below 4096 logits. us, whole rows
+  // and cut: 16 x 128256 33.3 and 8.4, 256 58.4 and 30.2, 1024 106.5 and 107.6; 256 x
+  // 32000 18.3 and 10.8.
   long long cuts = rows >= 2048 ? 1 : (2048 + rows - 1) / rows;
   if (cuts > (V + 4095) / 4096) cuts = (V + 4095) / 4096;
   const long long span = ((V + cuts - 1) / cuts + 7) / 8 * 8;

@@ -202,6 +202,35 @@ def test_infinite_logits_in_long_rows_gpu():
 
 
 @pytest.mark.gpu
+def test_parts_and_whole_rows_gpu():
+    """Rows of more than four parts, few and many, with masked logits."""
+    for rows in (2, 399, 401):
+        x, y, glp, gent = _inputs(rows, 40011, torch.bfloat16, "cuda", ignored=1)
+        x[:, 7::3] = -math.inf
+        live = y != IGNORE
+        y = torch.where(live, y // 3 * 3, y)
+        x.scatter_(1, y.clamp(min=0)[:, None], 1.0)
+        _check(x, y, glp, gent, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+def test_one_best_gpu(kind):
+    """The first of equal ones, of a row of the type's lowest value, of minus
+    infinity alone, and NaN before all."""
+    x = torch.full((6, 20003), torch.finfo(kind).min, dtype=kind, device="cuda")
+    x[1, [19999, 77, 20002]] = 3
+    x[2] = -math.inf
+    x[3] = -math.inf
+    x[3, 20002] = torch.finfo(kind).min
+    x[4, [700, 12345]] = math.nan
+    x[5, [0, 20002]] = -0.0
+    y = torch.zeros(6, dtype=torch.long, device="cuda")
+    ids = token_logprobs(x, y, top=1).top_ids.cpu()
+    assert ids.flatten().tolist() == [0, 77, 0, 20002, 700, 0]
+
+
+@pytest.mark.gpu
 def test_peaked_and_large_gpu():
     """Nearly sure rows keep the entropy's digits, large logits theirs."""
     for shift in (0.0, 1e4, -1e4):
