@@ -11,7 +11,7 @@
 // Every mask is an interval of keys for a query, lo and hi growing with the query,
 // and with that an interval of queries for a key (spans_kernel): a tile of either
 // is skipped, taken whole or compared element by element by the ends of its first
-// and last rows alone, and what is skipped costs nothing. Layout of the tiles,
+// and last rows alone, and what is skipped costs nothing. Layout of the products,
 // order of the contracted index and the two passes of the backward are those of
 // attention.hip, which says why.
 //
@@ -178,12 +178,22 @@ __device__ __forceinline__ void settle(s16x8 (&x)[N]) {
 }
 
 // ------------------------------------------------------------------ forward
+//
+// 4 waves of 32 query rows walk the keys that any of them sees, 32 or 64 a step, K and V
+// double-buffered in LDS by direct loads. Three workgroups a CU (two of heads of 64's
+// four), so that one's first loads and last stores lie behind another's products: a
+// document of a few hundred tokens is seven steps of a workgroup. Bound by the vector
+// unit (74% busy, and the matrix cores 36%, at the 2.0 GHz that the power leaves). us:
+// 1 x 8192 capped, 32 on 8 heads of 128 732 (751 TFLOP/s); nine documents in 4 x 4096 225
+// (385 of what is seen, 1.19 times that computed); 8 x 1999, eleven documents of 12
+// heads of 64 with the bias 56; 2 x 4096 capped, four with prefixes, 32 heads of 96 246.
+// The first kernel, eight waves and steps of 64, took 862, 263, 56 and 273.
 
 template <int D, int CAP, bool BIAS, int NW, int KB>
-__global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(const Args a,
-                                                         const int blocks,
-                                                         const int heads) {
-  constexpr int KT = KB / 32, DB = D / 32, KK = D / 16, QB = 32 * NW, TPB = 64 * NW;
+__global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(
+    const Args a, const int blocks, const int heads) {
+  constexpr int KT = KB / 32, DB = D / 32, KK = D / 16;
+  constexpr int QB = 32 * NW, TPB = 64 * NW;
   constexpr bool PLAIN = !CAP && !BIAS;
   using T = Tile<D, true>;
   __shared__ __attribute__((aligned(16))) short kt[2][KB * T::SC * 8];
@@ -405,6 +415,15 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(const Ar
 
 // ----------------------------------------------------------------- backward
 
+// Both passes compute S and dP again, as attention.hip's: every sum in registers and in
+// one order, no atomics. dQ goes first and leaves sum(do * o) for the other: a kernel for
+// these alone read do once more (54 us of the nine documents' 930 in all). Bound by the
+// matrix and vector units together (39 and 57 to 65% busy; waves of two or eight to a
+// tile, a half's products beside the other half's arithmetic or prefetched operands are
+// all slower). us, cases as above: dQ 1186 (696 TFLOP/s of its three products, 4 with what
+// a rounding leaves), 313, 65, 375; dK and dV 1345 and 47 for the splits' sums (790 of
+// four), 342, 78, 365.
+//
 // dK and dV: a wave owns 32 keys and walks the queries that see them.
 template <int D, int CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
@@ -771,10 +790,23 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const s16x8 sb = operand(dp, s);
+        // of capped scores what the rounding leaves as well: without it dQ was 0.0025
+        // off 64 bits, 1.5 times its own rounding's 0.0017 (now the same), with it the
+        // pass over 1 x 8192 takes 1186 us for 1011. Without a cap 0.0024, as is dK.
+        s16x8 lb;
+        if (CAP) {
+          f32x16 left;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
-          acc[db] =
-              mfma(T::cols(kt[cur], 32 * t + 16 * s, db, ca), sb, acc[db]);
+          for (int r = 0; r < 8; ++r)
+            left[8 * s + r] = dp[8 * s + r] - value(sb[r]);
+          lb = operand(left, s);
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const s16x8 kc = T::cols(kt[cur], 32 * t + 16 * s, db, ca);
+          acc[db] = mfma(kc, sb, acc[db]);
+          if (CAP) acc[db] = mfma(kc, lb, acc[db]);
+        }
       }
     }
     arrive();
@@ -834,7 +866,8 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
 // s .. max(i + 1, s + p) - 1 (causal) or s .. e - 1, a key j is seen by the queries
 // from j on, or of the prefix from s on. Rows of no document see nothing and stand
 // at themselves, which keeps all four growing. A thread a row; the document's ends
-// past the workgroup's own rows are looked for 4096 rows at a time.
+// past the workgroup's own rows are looked for 4096 rows at a time. 3 to 7 us (4 x 4096,
+// 1 x 8192), once a batch.
 
 constexpr int ST = 1024, FAR = 4 * ST;
 
@@ -946,7 +979,7 @@ int launch(const Args& a, int splits, hipStream_t s) {
   // documents in 4 x 4096 258 / 230, heads of 96 273 / 250); heads of 64 hold four
   // either way (59 / 62). Eight waves that share the tiles took 883, 305, 296 and 64.
   constexpr int KB = D == 64 ? 64 : 32;
-#define GO(C, W)                      \
+#define GO(C, W)                              \
   (splits ? launch_bwd<D, C, W>(a, splits, s) \
           : launch_fwd<D, C, W, 4, KB>(a, s))
   if (a.cap == 0.f) return bias ? GO(NONE, true) : GO(NONE, false);

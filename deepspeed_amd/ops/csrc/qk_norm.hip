@@ -9,7 +9,9 @@
 // lane, chosen so that the pairs that turn together lie in one lane (`Places`). A
 // wave stays with one token and takes its heads in turn, so that the angles are read
 // once a token and not once a head. All in fp32, rounded once at the end. Bound by
-// the stream of heads in and out.
+// the stream of heads in and out: 8192 tokens, 32 and 8 heads of 128, bf16: 34 us forward
+// (168 MB, 4.9 TB/s), 60 backward (252 MB, 4.2 TB/s) and 4 for the weights' sums; 100
+// without the next heads' loads in flight. 16 tokens 4.6 us, a launch.
 
 #include "ds_kernels.h"
 
