@@ -84,6 +84,27 @@ bool wants_grad(const Tensor& t) {
   return at::GradMode::is_enabled() && t.requires_grad();
 }
 
+// An eager graph that lives keeps the place of its leaves' gradients on the stream it
+// was made on. On the default one, which no capture can take in, a captured backward
+// of the same leaves ends the process: such a forward is refused.
+void check_capture(const char* what,
+                   std::initializer_list<const Tensor*> inputs) {
+  for (const auto* t : inputs) {
+    if (!wants_grad(*t) || !t->is_leaf()) continue;
+    const auto place = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!place) continue;
+    const auto kept = place->stream();
+    if (!kept || kept->id() != 0) continue;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const auto now = c10::hip::getCurrentHIPStream(t->device().index());
+    TORCH_CHECK(hipStreamIsCapturing(now.stream(), &status) == hipSuccess &&
+                    status == hipStreamCaptureStatusNone,
+                what, ": an eager graph of the same leaves lives, which a capture "
+                "with gradients cannot take in; end it before, or give the capture "
+                "leaves of its own");
+  }
+}
+
 at::Tensor packed_spans(at::Tensor ids, Opt prefix, bool causal) {
   const OneDevice on("packed_rows", ids, prefix);
   const bool wide = ids.scalar_type() == at::kLong;
@@ -147,7 +168,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_fwd(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
         lse.data_ptr<float>(), with_rest ? rest.data_ptr() : nullptr, nullptr,
         nullptr, nullptr, nullptr, nullptr, nullptr, 0, a.spans, a.slopes,
-        a.strides.data(), a.B, a.S, a.H, a.Hkv, a.D, causal, (float)scale, (float)cap, cur_stream());
+        a.strides.data(), a.B, a.S, a.H, a.Hkv, a.D, causal, (float)scale,
+        (float)cap, cur_stream());
     TORCH_CHECK(e == 0, "masked_attention: launch failed, hipError_t ", e);
   }
   return {o, lse, rest};
@@ -176,8 +198,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> masked_attn_bwd(
     const int e = ds_masked_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
         lse.data_ptr<float>(), rest.data_ptr(), dout.data_ptr(), dq.data_ptr(),
-        dk.data_ptr(), dv.data_ptr(), stat.data_ptr<float>(), part.data_ptr<float>(), splits,
-        a.spans, a.slopes, a.strides.data(), a.B, a.S, a.H, a.Hkv, a.D, causal,
+        dk.data_ptr(), dv.data_ptr(), stat.data_ptr<float>(),
+        part.data_ptr<float>(), splits, a.spans, a.slopes, a.strides.data(), a.B, a.S, a.H, a.Hkv, a.D, causal,
         (float)scale, (float)cap, cur_stream());
     TORCH_CHECK(e == 0, "masked_attention: launch failed, hipError_t ", e);
   }
@@ -276,6 +298,7 @@ Tensor masked_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   const Opt slopes = slopes_of(alibi_slopes, q, "masked_attention");
   TORCH_CHECK_VALUE(k.device() == q.device() && v.device() == q.device(),
                     "masked_attention: tensors on different devices");
+  check_capture("masked_attention", {&q, &k, &v});
   return MaskedAttention::apply(
       q, k, v, spans, slopes, causal,
       scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3)), softcap,
@@ -515,6 +538,9 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k,
   TORCH_CHECK_VALUE(here && (!positions.has_value() ||
                              positions->device() == q.device()),
                     "qk_norm_rope: tensors on different devices");
+  TORCH_CHECK_VALUE(!cos.requires_grad() && !sin.requires_grad(),
+                    "qk_norm_rope: cos and sin have no gradient");
+  check_capture("qk_norm_rope", {&q, &k, &q_weight, &k_weight});
   Opt pos;
   if (positions.has_value()) pos = positions->contiguous();
   const auto c = cos.contiguous(), s = sin.contiguous();
@@ -666,6 +692,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(
                     top, " of ", V);
   TORCH_CHECK_VALUE(logits.device() == tokens.device(),
                     "token_logprobs: tensors on different devices");
+  check_capture("token_logprobs", {&logits});
   const auto y = TokenLogprobs::apply(
       logits, tokens.to(at::kLong).contiguous(), top, ignore_index);
   return {y[0], y[1], y[2], y[3]};

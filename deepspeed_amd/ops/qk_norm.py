@@ -79,5 +79,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     if any(t is not None and t.device != q.device
            for t in (k, q_weight, k_weight, cos, sin, positions)):
         raise ValueError("qk_norm_rope: tensors on different devices")
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("qk_norm_rope: cos and sin have no gradient")
     how = cos, sin, positions, eps, layout, one_plus
     return _torch_heads(q, q_weight, *how), _torch_heads(k, k_weight, *how)

@@ -168,3 +168,45 @@ def test_inference_mode_and_autocast_gpu():
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     _loss(got, torch.ones_like(got.logprobs)).backward()
     assert all(torch.isfinite(p.grad).all() for p in model.parameters())
+
+
+@pytest.mark.gpu
+def test_capture_beside_an_eager_graph_gpu():
+    """Refused while an eager graph of the same leaves lives; sound after its end."""
+    def leaf(*shape):
+        return torch.randn(*shape, device="cuda").bfloat16().requires_grad_()
+
+    q, k, v = leaf(1, 70, 4, 64), leaf(1, 70, 2, 64), leaf(1, 70, 2, 64)
+    qw, kw = leaf(64), leaf(64)
+    cos, sin = rope_tables(64, 70, device="cuda")
+    x, y = leaf(5, 999), torch.arange(5, device="cuda")
+    calls = [(lambda: masked_attention(q, k, v), (q, k, v)),
+             (lambda: qk_norm_rope(q, k, qw, kw, cos, sin)[0], (q, k, qw, kw)),
+             (lambda: token_logprobs(x, y).logprobs, (x,))]
+    for call, leaves in calls:
+        out = call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = torch.zeros(3, device="cuda")
+            with pytest.raises(RuntimeError, match="eager graph"):
+                call()
+            with torch.no_grad():
+                there = call()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(there, out) and not held.any()
+        ones = torch.ones_like(out)
+        want = torch.autograd.grad(out, leaves, ones)
+        del out, graph, there
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(call(), leaves, ones)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(call(), leaves, ones)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

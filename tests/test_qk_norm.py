@@ -124,6 +124,23 @@ def test_refusals():
         qk_norm_rope(q, k, qw, kw, cos[:2], sin[:2])
 
 
+def _constant_angles(device):
+    ins, _ = _inputs(2, 3, 4, 2, 64, 64, torch.float32, device)
+    for i in (4, 5):
+        leaves = [t.clone().requires_grad_(j == i) for j, t in enumerate(ins[:6])]
+        with pytest.raises(ValueError, match="no gradient"):
+            qk_norm_rope(*leaves, ins[6])
+
+
+def test_constant_angles_cpu():
+    _constant_angles("cpu")
+
+
+@pytest.mark.gpu
+def test_constant_angles_gpu():
+    _constant_angles("cuda")
+
+
 def _bad_positions(device):
     ins, dy = _inputs(2, 5, 4, 2, 64, 32, torch.float32, device)
     for bad in (-1, 64, 2 ** 31 - 1, -2 ** 31):
