@@ -62,8 +62,8 @@ struct Sums {
     if (t > m) {
       const float d2 = (m - t) * LOG2E;
       const float f = power(d2);
-      // of nothing seen yet, d2 is as good as -inf
-      u = s > 0.f ? f * __builtin_fmaf(s, d2, u) : 0.f;
+      // what has no share beside t adds nothing: s d2 may be past all numbers
+      u = f > 0.f ? f * __builtin_fmaf(s, d2, u) : 0.f;
       s *= f;
       m = t;
     }
@@ -123,7 +123,7 @@ __device__ __forceinline__ float lanes_sum(float x) {
 __device__ __forceinline__ void join_lanes(Sums& a) {
   const float m = lanes_max(a.m);
   const float d2 = (a.m - m) * LOG2E, f = power(d2);
-  float u = a.s > 0.f ? f * __builtin_fmaf(a.s, d2, a.u) : 0.f;
+  float u = f > 0.f ? f * __builtin_fmaf(a.s, d2, a.u) : 0.f;     // as raise
   float s = a.s * f;
   if (a.s != a.s) s = u = a.s;
   a.s = lanes_sum(s);

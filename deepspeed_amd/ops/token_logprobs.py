@@ -32,8 +32,8 @@ def _torch_logprobs(logits, tokens, top, ignore_index):
     known = (tokens >= 0) & (tokens < V)
     x = x.masked_fill(~live[..., None], 0.0)
     lp = torch.log_softmax(x, -1)
-    # a logit of -inf has no share
-    none = lp == float("-inf")
+    # a logit of no share adds nothing, though its logarithm be past all numbers
+    none = lp.exp() == 0
     some = lp.masked_fill(none, 0.0)
     share = torch.where(none, 0.0, some.exp() * some)
     entropy = torch.where(live, -share.sum(-1), 0.0)

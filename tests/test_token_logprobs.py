@@ -333,3 +333,37 @@ def test_wide_gradient_gpu():
     torch.testing.assert_close(dx[-5:].float(), dsmall.float(), rtol=2.0 ** -7,
                                atol=1e-7)
     torch.testing.assert_close(got.logprobs[-5:], want.logprobs, rtol=1e-6, atol=1e-5)
+
+
+# What programs write over logits that may not be sampled, besides -inf.
+MASKS = [-1e30, -1e36, -1.7e38, -2.5e38]
+
+
+def _masked(kind, mask, rows, V, device):
+    """Logits with a stretch of whole parts and single ones masked, tokens that are
+    not, and gradients."""
+    x, y, glp, gent = _inputs(rows, V, kind, device, seed=3)
+    x[:, :V * 2 // 5] = mask
+    x[:, V // 2::3] = mask
+    y = torch.where(y == IGNORE, y, V // 2 + 1)
+    return x, y, glp, gent
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", MASKS)
+def test_masked_logits_cpu(mask, kind):
+    _check(*_masked(kind, mask, 3, 1003, "cpu"), top=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("rows", [3, 420])
+def test_masked_logits_gpu(rows, mask, kind):
+    """A thread, a part or a chunk that saw masked logits alone adds nothing to the
+    entropy of the rest: rows by parts and whole ones."""
+    for top in (0, 3):
+        _check(*_masked(kind, mask, rows, 40011, "cuda"), top)
+    low = torch.finfo(kind).min
+    for masked in (low, low / 2):
+        _check(*_masked(kind, masked, rows, 40011, "cuda"))
