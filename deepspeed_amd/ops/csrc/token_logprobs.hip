@@ -19,7 +19,8 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr float LOWEST = -3.0e38f;     // a maximum before anything was seen
+// A maximum before anything was seen: no finite logit lies below it.
+constexpr float LOWEST = -__FLT_MAX__;
 constexpr int CT = 256;                // threads of a workgroup
 constexpr int HELD = 32;               // logits that a thread holds
 constexpr int PART = CT * HELD;        // logits of a part of a row

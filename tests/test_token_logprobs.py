@@ -357,13 +357,41 @@ def test_masked_logits_cpu(mask, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("mask", MASKS)
-@pytest.mark.parametrize("rows", [3, 420])
-def test_masked_logits_gpu(rows, mask, kind):
+@pytest.mark.parametrize("mask", MASKS + ["lowest", "half of it"])
+@pytest.mark.parametrize("V", [24003, 40011])
+def test_masked_logits_gpu(V, mask, kind):
     """A thread, a part or a chunk that saw masked logits alone adds nothing to the
     entropy of the rest: rows by parts and whole ones."""
-    for top in (0, 3):
-        _check(*_masked(kind, mask, rows, 40011, "cuda"), top)
     low = torch.finfo(kind).min
-    for masked in (low, low / 2):
-        _check(*_masked(kind, masked, rows, 40011, "cuda"))
+    mask = {"lowest": low, "half of it": low / 2}.get(mask, mask)
+    for top in (0, 3):
+        _check(*_masked(kind, mask, 3, V, "cuda"), top)
+
+
+def _lowest_rows(kind, rows, V, device):
+    """Rows masked from end to end, with the type's lowest value and with others near
+    it, and some that are not."""
+    x, y, glp, gent = _inputs(rows, V, kind, device, seed=4, ignored=0)
+    low = torch.finfo(kind).min
+    x[0] = low
+    x[1, ::2], x[1, 1::2] = low, low * 0.95
+    x[1, 5] = low * 0.9
+    x[2] = low / 2
+    y[:3] = 5
+    return x, y, glp, gent
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_lowest_rows_cpu(kind):
+    """Every token of a row of one value is as probable, whatever the value."""
+    got, _ = _check(*_lowest_rows(kind, 4, 1003, "cpu"))
+    assert got.logprobs[0].item() == pytest.approx(-math.log(1003), rel=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("V", [24003, 40011])
+def test_lowest_rows_gpu(V, kind):
+    for top in (0, 2):
+        got, _ = _check(*_lowest_rows(kind, 4, V, "cuda"), top)
+        assert got.logprobs[0].item() == pytest.approx(-math.log(V), rel=1e-5)
