@@ -151,11 +151,17 @@ __device__ __forceinline__ void join_waves(Sums& a, float (*lds)[3]) {
   a = w;
 }
 
+// A logit's log probability in a row of maximum m and sum of 2^logs: the difference is not
+// scaled there and back, which would lose masked logits to -inf.
+__device__ __forceinline__ float logprob(float x, float m, float logs) {
+  return (x - m) - logs * LN2;
+}
+
 // What a row comes to. A token outside of the row has no log probability.
 __device__ __forceinline__ void finish(const Sums& a, float xy, bool known,
                                        float* lp, float* ent, float* stat) {
   const float logs = __builtin_amdgcn_logf(a.s);       // log2
-  *lp = known ? ((xy - a.m) * LOG2E - logs) * LN2 : __builtin_nanf("");
+  *lp = known ? logprob(xy, a.m, logs) : __builtin_nanf("");
   *ent = (logs - a.u / a.s) * LN2;
   stat[0] = a.m;
   stat[1] = logs;
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(64) void join_kernel(
   }
   __syncthreads();
   places(held, n, top, [&](int r, Rated e) {
-    top_lp[out + r] = ((logit_of(e) - a.m) * LOG2E - logs) * LN2;
+    top_lp[out + r] = logprob(logit_of(e), a.m, logs);
     top_ids[out + r] = id_of(e);
   });
 }

@@ -395,3 +395,30 @@ def test_lowest_rows_gpu(V, kind):
     for top in (0, 2):
         got, _ = _check(*_lowest_rows(kind, 4, V, "cuda"), top)
         assert got.logprobs[0].item() == pytest.approx(-math.log(V), rel=1e-5)
+
+
+def _masked_tokens(kind, rows, V, device, top):
+    """Tokens of masked logits, and best ones among which are masked ones."""
+    for mask in (torch.finfo(kind).min, torch.finfo(kind).min * 0.8):
+        x, y, glp, gent = _masked(kind, mask, rows, V, device)
+        x[1:] = mask
+        x[1:, [3, V - 1]] = 1.0
+        y[:2], y[2:] = 7, 3
+        got, _ = _check(x, y, glp, gent, top)
+        assert torch.isfinite(got.logprobs).all()
+        assert torch.isfinite(got.top_logprobs).all()
+        # what a token was less probable under is a number, too
+        assert (got.logprobs[:2] - got.logprobs[:2]).abs().sum() == 0
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_masked_tokens_cpu(kind):
+    _masked_tokens(kind, 4, 1003, "cpu", 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("V", [24003, 40011])
+def test_masked_tokens_gpu(V, kind):
+    for top in (0, 4):
+        _masked_tokens(kind, 4, V, "cuda", top)
