@@ -499,7 +499,7 @@ __global__ __launch_bounds__(CT) void grad_kernel(
   T* d = dx + (long long)row * V;
   const float m = stat[2 * row], logs = stat[2 * row + 1];
   float g = glp ? glp[row] : 0.f;
-  if (y < 0 || y >= V) g = __builtin_nanf("");
+  if (glp && (y < 0 || y >= V)) g = __builtin_nanf("");
   const float h = gent ? gent[row] : 0.f;
   // g + h (x - m - log s + entropy) = base + h ln 2 (d2), d2 as below
   const float slope = h * LN2, base = __builtin_fmaf(h, ent[row], g);

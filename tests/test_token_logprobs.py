@@ -407,8 +407,6 @@ def _masked_tokens(kind, rows, V, device, top):
         got, _ = _check(x, y, glp, gent, top)
         assert torch.isfinite(got.logprobs).all()
         assert torch.isfinite(got.top_logprobs).all()
-        # what a token was less probable under is a number, too
-        assert (got.logprobs[:2] - got.logprobs[:2]).abs().sum() == 0
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -422,3 +420,27 @@ def test_masked_tokens_cpu(kind):
 def test_masked_tokens_gpu(V, kind):
     for top in (0, 4):
         _masked_tokens(kind, 4, V, "cuda", top)
+
+
+def _entropy_alone(device, V):
+    """The entropy knows nothing of the token: nor does its gradient, whatever the
+    token is, where no log probability has one."""
+    x, y, _, gent = _inputs(6, V, torch.float32, device, ignored=0)
+    grads = []
+    for tokens in (y, torch.tensor([V, -1, -(2 ** 40), 2 ** 40, V + 7, 0]).to(device)):
+        leaf = x.detach().requires_grad_()
+        got = token_logprobs(leaf, tokens)
+        grads += torch.autograd.grad(got.entropy, leaf, gent)
+    assert got.logprobs[:5].isnan().all() and torch.isfinite(got.entropy).all()
+    assert torch.isfinite(grads[0]).all() and torch.equal(*grads)
+    _check(x, y, torch.zeros_like(gent), gent)
+
+
+def test_entropy_alone_cpu():
+    _entropy_alone("cpu", 103)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [103, 40011])
+def test_entropy_alone_gpu(V):
+    _entropy_alone("cuda", V)
