@@ -40,10 +40,16 @@ def _torch_logprobs(logits, tokens, top, ignore_index):
     got = lp.gather(-1, torch.where(known, tokens, 0)[..., None])[..., 0]
     got = got * torch.where(known | ~live, 1.0, float("nan")).to(got.dtype)
     got = torch.where(live, got, 0.0)
-    # NaN above all, as numbers that are equal in order of their ids
-    order = torch.sort(torch.where(x != x, float("inf"), x).detach(), dim=-1,
-                       descending=True, stable=True).indices[..., :top] \
-        if top else tokens.new_empty(*tokens.shape, 0)
+    order = tokens.new_empty(*tokens.shape, 0)
+    if top:
+        # NaN above all, infinity among it, as numbers that are equal in order of their
+        # ids: by values, then by which are none
+        nan = x.detach() != x.detach()
+        order = torch.sort(x.detach().masked_fill(nan, 0.0), dim=-1, descending=True,
+                           stable=True).indices
+        first = torch.sort(nan.gather(-1, order).to(torch.int8), dim=-1,
+                           descending=True, stable=True).indices
+        order = order.gather(-1, first)[..., :top]
     best = lp.detach().gather(-1, order)
     return TokenLogprobs(got, entropy,
                          torch.where(live[..., None], best, float("-inf")),

@@ -444,3 +444,23 @@ def test_entropy_alone_cpu():
 @pytest.mark.parametrize("V", [103, 40011])
 def test_entropy_alone_gpu(V):
     _entropy_alone("cuda", V)
+
+
+def _nan_above_infinity(device):
+    inf, nan = math.inf, math.nan
+    x = torch.tensor([[0.0, inf, nan, 1.0, nan, inf], [inf, nan, inf, -inf, 0.0, 1.0]],
+                     device=device)
+    y = torch.zeros(2, dtype=torch.long, device=device)
+    want = [[2, 4, 1, 5, 3, 0], [1, 0, 2, 5, 4, 3]]
+    for top in (1, 3, 6):
+        ids = token_logprobs(x, y, top=top).top_ids.tolist()
+        assert ids == [row[:top] for row in want]
+
+
+def test_nan_above_infinity_cpu():
+    _nan_above_infinity("cpu")
+
+
+@pytest.mark.gpu
+def test_nan_above_infinity_gpu():
+    _nan_above_infinity("cuda")
