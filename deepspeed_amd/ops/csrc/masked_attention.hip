@@ -55,15 +55,15 @@ struct Span {
   int lo, hi;
 };
 
-// Keys that query i sees, or queries that see key i, whatever the spans hold
-// inside the row.
+// Keys that query i sees, or queries that see key i: inside the row whatever the spans
+// hold, both ends, since a difference of ends anywhere may wrap to a positive one.
 __device__ __forceinline__ Span span(const Args& a, int b, int i, bool key) {
   Span s;
   if (a.spans != nullptr) {
     const long long n = (long long)a.B * a.S;
     const int* p = a.spans + (key ? 2 * n : 0) + (long long)b * a.S + i;
-    s.lo = max(p[0], 0);
-    s.hi = min(p[n], a.S);
+    s.lo = min(max(p[0], 0), a.S);
+    s.hi = min(max(p[n], 0), a.S);
   } else {
     s.lo = key && a.causal ? i : 0;
     s.hi = !key && a.causal ? i + 1 : a.S;

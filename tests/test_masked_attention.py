@@ -660,3 +660,25 @@ def test_seen_infinities_gpu():
         near(name, x, slice(251, None))
     near("dq", got[1], slice(250))
     assert got[1][0, 250].isnan().all() and got[2][0, 200:251].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [True, False])
+def test_wild_spans_gpu(queries):
+    """Spans whose ends lie anywhere are those inside of the row: forward and both
+    passes of the backward read and write nothing else."""
+    ends = [-2 ** 31, -1, 0, 3, 69, 70, 2 ** 31 - 2, 2 ** 31 - 1]
+    S = 70
+    q, k, v, do = _inputs(1, S, 2, 1, 64, "cuda", seed=19)
+    for lo in ends:
+        for hi in ends:
+            spans = torch.tensor([0, S, 0, S], dtype=torch.int32).repeat(S, 1).t()
+            spans[0 if queries else 2], spans[1 if queries else 3] = lo, hi
+            spans = spans.contiguous().view(4, 1, S)
+            got = _grads(q, k, v, do, PackedRows(spans.cuda(), False))
+            want = _grads(q, k, v, do, PackedRows(spans.clamp(0, S).cuda(), False))
+            # (keys seen by queries that see nothing have no gradient that is a number)
+            for x, y in zip(got, want):
+                torch.testing.assert_close(x, y, rtol=0, atol=0, equal_nan=True)
+            if queries and max(lo, 0) >= min(hi, S):
+                assert not got[0].any() and not got[1].any()
