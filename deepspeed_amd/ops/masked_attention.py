@@ -76,30 +76,62 @@ def packed_rows(document_ids: torch.Tensor,
     return PackedRows(spans, causal)
 
 
-def _torch_attention(q, k, v, spans, causal, scale, softcap, slopes):
-    """The formulas on whole score matrices, in fp32 (fp64 for fp64)."""
-    B, S, H, D = q.shape
-    G = H // k.shape[2]
-    wide = torch.float64 if q.dtype is torch.float64 else torch.float32
-    qt, kt, vt = (x.to(wide).transpose(1, 2) for x in (q, k, v))
-    kt, vt = (x.repeat_interleave(G, 1) for x in (kt, vt))
-    t = (qt @ kt.transpose(2, 3).contiguous()) * scale
+def _formulas(q, k, v, far, seen, scale, softcap, slopes):
+    """q [B, Sq, H, D], k and v [B, Sk, Hkv, D] of one type, far [Sq, Sk] the distances,
+    ``seen`` [B or 1, 1, Sq, Sk] or None (all)."""
+    G = q.shape[2] // k.shape[2]
+    q, k, v = (x.transpose(1, 2) for x in (q, k, v))
+    k, v = (x.repeat_interleave(G, 1) for x in (k, v))
+    t = (q @ k.transpose(2, 3).contiguous()) * scale
     if softcap:
         t = torch.tanh(t / softcap) * softcap
-    at = torch.arange(S, device=q.device)
     if slopes is not None:
-        t = t - slopes.to(wide).view(H, 1, 1) * (at[:, None] - at).abs()
-    if spans is not None:
-        lo, hi = (x[:, None, :, None] for x in spans[:2])
-        seen = (at >= lo) & (at < hi)
-    else:
-        seen = at <= at[:, None] if causal else at == at
+        t = t - slopes.to(t.dtype).view(-1, 1, 1) * far
+    if seen is None:
+        return (torch.softmax(t, -1) @ v).transpose(1, 2)
     t = t.masked_fill(~seen, -math.inf)
     top = t.amax(-1, keepdim=True).detach()
-    p = torch.exp(t - torch.where(seen.any(-1, keepdim=True), top, 0.0))
+    some = seen.any(-1, keepdim=True)
+    p = torch.exp(t - torch.where(some, top, 0.0))
     p = torch.where(seen, p, 0.0)
-    p = p / torch.where(seen.any(-1, keepdim=True), p.sum(-1, keepdim=True), 1.0)
-    return (p @ vt).transpose(1, 2).to(q.dtype)
+    p = p / torch.where(some, p.sum(-1, keepdim=True), 1.0)
+    return (p @ v).transpose(1, 2)
+
+
+def _torch_attention(q, k, v, spans, causal, scale, softcap, slopes):
+    """The formulas in fp32 (fp64 for fp64), on whole score matrices. What is hidden is
+    in no sum, as in the kernels: rows of no use count as 0, and if others are not finite
+    each query goes through its own keys alone. Not so where there are no values to look
+    at, under a transform, and not for gradients that come in so to rows of use."""
+    B, S, _, _ = q.shape
+    kind, wide = q.dtype, torch.float64 if q.dtype is torch.float64 else torch.float32
+    q, k, v = (x.to(wide) for x in (q, k, v))
+    at = torch.arange(S, device=q.device)
+    far = (at[:, None] - at).abs()
+    how = scale, softcap, slopes
+    if spans is None and not causal:
+        return _formulas(q, k, v, far, None, *how).to(kind)
+    if spans is not None:
+        lo, hi, klo, khi = spans[..., None]
+        seen = ((at >= lo) & (at < hi))[:, None]
+        used = (lo < hi)[..., None]
+        q = torch.where(used, q, 0.0)
+        k, v = (torch.where((klo < khi)[..., None], x, 0.0) for x in (k, v))
+    else:
+        seen = (at <= at[:, None])[None, None]
+        used = torch.ones_like(at, dtype=torch.bool)[:, None, None]
+    if torch.compiler.is_compiling() or not untransformed() or q.is_meta or \
+            all(bool(torch.isfinite(x).all()) for x in (q, k, v)):
+        o = _formulas(q, k, v, far, seen, *how)
+    else:
+        ends = torch.stack([0 * at, at + 1], -1).expand(B, S, 2) if spans is None \
+            else spans[:2].permute(1, 2, 0).clamp(0, S)
+        rows = [_formulas(q[b:b + 1, i:i + 1], k[b:b + 1, lo:hi], v[b:b + 1, lo:hi],
+                          far[i:i + 1, lo:hi], None, *how)
+                if lo < hi else torch.zeros_like(q[b:b + 1, i:i + 1])
+                for b, row in enumerate(ends.tolist()) for i, (lo, hi) in enumerate(row)]
+        o = torch.cat(rows, 1).view(q.shape)
+    return torch.where(used, o, 0.0).to(kind)
 
 
 def _checked_slopes(alibi_slopes, q, what):

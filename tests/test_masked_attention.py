@@ -177,6 +177,49 @@ def test_formulas_cpu(causal, cap, bias):
         lambda *x: masked_attention(*x, rows, **how), (q, k, v))
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (10.0, True)])
+def test_hidden_infinities_cpu(value, cap, bias):
+    """What a query does not see is not in its row nor in its gradients: padding,
+    another document's keys, values and queries, a later token."""
+    ids = _ids([[7, 6, -3], [-3, 5, 8]])
+    seen = _seen(ids, None, True)
+    slopes = torch.tensor([0.5, 0.1, 0.0, 2.0]) if bias else None
+    how = dict(scale=0.3, softcap=cap, alibi_slopes=slopes)
+    g = torch.Generator().manual_seed(7)
+    q, k, v, do = (torch.randn(2, 16, h, 4, generator=g, dtype=torch.float64)
+                   for h in (4, 2, 2, 4))
+    pad = ids < 0
+    for x in (q, k, v, do):
+        x[pad] = value
+    rows = packed_rows(ids)
+    want, _ = _reference(q, k, v, do, seen, 0.3, cap, slopes)
+    for x, y in zip(_grads(q, k, v, do, rows, **how), want):
+        torch.testing.assert_close(x, y, rtol=1e-9, atol=1e-12)
+        assert (x[pad] == 0).all()
+    # one of the first document, seen by its last 2 tokens only
+    other = torch.ones(2, 16, dtype=torch.bool)
+    other[0, :7] = False
+    well = other.clone()
+    well[0, :5] = True
+    for i in range(3):
+        sick = [x.clone() for x in (q, k, v)]
+        sick[i][0, 5] = value
+        got = _grads(*sick, do, rows, **how)
+        for x, y, part in zip(got, want, (well, other, other, other)):
+            torch.testing.assert_close(x[part], y[part], rtol=1e-9, atol=1e-12)
+        if i == 2:
+            assert not torch.isfinite(got[0][0, 5:7]).any()
+    # without documents: later tokens are as hidden
+    q, k, v, do = (torch.where(pad[..., None, None], 0.0, x) for x in (q, k, v, do))
+    want = _grads(q, k, v, do, None, **how)
+    for x in (k, v):
+        x[:, 12] = value
+    for i, (x, y) in enumerate(zip(_grads(q, k, v, do, None, **how), want)):
+        if i < 2:
+            torch.testing.assert_close(x[:, :12], y[:, :12], rtol=1e-9, atol=1e-12)
+
+
 def test_refusals():
     q, k, v, _ = _inputs(2, 6, 4, 2, 64, "cpu")
     ids = _ids([[6], [2, 4]])
