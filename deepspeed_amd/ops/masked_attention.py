@@ -109,7 +109,7 @@ def _torch_attention(q, k, v, spans, causal, scale, softcap, slopes):
     at = torch.arange(S, device=q.device)
     far = (at[:, None] - at).abs()
     how = scale, softcap, slopes
-    if spans is None and not causal:
+    if S == 0 or spans is None and not causal:
         return _formulas(q, k, v, far, None, *how).to(kind)
     if spans is not None:
         lo, hi, klo, khi = spans[..., None]

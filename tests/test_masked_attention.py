@@ -220,6 +220,18 @@ def test_hidden_infinities_cpu(value, cap, bias):
             torch.testing.assert_close(x[:, :12], y[:, :12], rtol=1e-9, atol=1e-12)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_no_tokens_cpu(causal):
+    for B, S in ((2, 0), (0, 5), (0, 0)):
+        q, k, v = (torch.empty(B, S, h, 4, requires_grad=True) for h in (4, 2, 2))
+        ids = torch.empty(B, S, dtype=torch.int64)
+        for rows in (None, packed_rows(ids, causal=causal)):
+            o = masked_attention(q, k, v, rows, causal=causal, softcap=1.0)
+            assert o.shape == q.shape
+            grads = torch.autograd.grad(o.sum(), (q, k, v))
+            assert [x.shape for x in grads] == [x.shape for x in (q, k, v)]
+
+
 def test_refusals():
     q, k, v, _ = _inputs(2, 6, 4, 2, 64, "cpu")
     ids = _ids([[6], [2, 4]])
