@@ -69,7 +69,11 @@ def packed_rows(document_ids: torch.Tensor,
         if prefix_lens.device != document_ids.device:
             raise ValueError("packed_rows: tensors on different devices")
     if document_ids.is_cuda and get_ext() is not None and untransformed():
-        prefix = None if prefix_lens is None else prefix_lens.int().contiguous()
+        prefix = prefix_lens
+        if prefix is not None:
+            if prefix.dtype is torch.int64:       # no length wraps to another
+                prefix = prefix.clamp(0, document_ids.shape[1]).int()
+            prefix = prefix.contiguous()
         spans = get_ext().packed_spans(document_ids.contiguous(), prefix, causal)
     else:
         spans = _torch_spans(document_ids, prefix_lens, causal)

@@ -737,3 +737,21 @@ def test_wild_spans_gpu(queries):
                 torch.testing.assert_close(x, y, rtol=0, atol=0, equal_nan=True)
             if queries and max(lo, 0) >= min(hi, S):
                 assert not got[0].any() and not got[1].any()
+
+
+def _long_prefixes(device):
+    """Lengths past 32 bits mean all of the document, or nothing below 0."""
+    ids = _ids([[5, 4, 3], [6, 6]]).to(device)
+    lens = torch.tensor([[2 ** 31, 2 ** 32 + 1, -2 ** 32 + 2], [2 ** 63 - 1, -2 ** 63, 2]])
+    got = packed_rows(ids, lens.to(device))
+    want = packed_rows(ids, lens.clamp(0, 12).int().to(device))
+    assert torch.equal(got.spans, want.spans)
+
+
+def test_long_prefixes_cpu():
+    _long_prefixes("cpu")
+
+
+@pytest.mark.gpu
+def test_long_prefixes_gpu():
+    _long_prefixes("cuda")
