@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <tuple>
 
 extern "C" int ds_packed_spans(const void* ids, int wide, const int* prefix,
@@ -310,6 +311,15 @@ Tensor aligned(const Tensor& t) {     // contiguous, on 16 bytes
   return (uintptr_t)x.data_ptr() % 16 == 0 ? x : x.clone();
 }
 
+// Numbers of 64 bits in 32: one that does not fit is the nearest that does, which is as
+// far outside of any pool or table, and not some other's that it would wrap to.
+Tensor in_32_bits(const Tensor& t) {
+  return (t.scalar_type() == at::kLong
+              ? t.clamp(std::numeric_limits<int>::min(),
+                        std::numeric_limits<int>::max())
+              : t).to(at::kInt).contiguous();
+}
+
 // Parts of each request, of whose keys the table's width is all that the host knows. us
 // from cold caches, whole / in these parts, groups of heads times requests by keys:
 //   up to 512 keys whole: 8 x 350 8.7, in two parts 10.0
@@ -369,8 +379,7 @@ Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
   const Opt slopes = slopes_of(alibi_slopes, q_, what);
   const OneDevice on(what, q_);
   const auto q = aligned(q_), kpool = aligned(kpool_), vpool = aligned(vpool_);
-  const auto table = table_.to(at::kInt).contiguous();
-  const auto lens = lens_.to(at::kInt).contiguous();
+  const auto table = in_32_bits(table_), lens = in_32_bits(lens_);
   const int64_t n = q.size(0), H = q.size(1), Hkv = kpool.size(1);
   const int64_t BS = kpool.size(2), groups = n * Hkv;
   auto o = at::empty_like(q);

@@ -755,3 +755,32 @@ def test_long_prefixes_cpu():
 @pytest.mark.gpu
 def test_long_prefixes_gpu():
     _long_prefixes("cuda")
+
+
+def _long_pages(device):
+    """Blocks and lengths past 32 bits are not others that they would wrap to."""
+    q, kp, vp, table, lens = _decode_inputs([20, 32, 9], 4, 2, 16, device)
+    table, lens = table.clamp(min=0).long(), lens.long()
+    o = paged_decode_attention(q, kp, vp, table, lens, softcap=5.0)
+    for far in (2 ** 32, -2 ** 32, 2 ** 62):
+        sick = table.clone()
+        sick[1, 1] += far
+        got = paged_decode_attention(q, kp, vp, sick, lens, softcap=5.0)
+        assert got[1].isnan().all() and torch.equal(got[::2], o[::2])
+    most = lens.clone()
+    most[0] = table.shape[1] * 16
+    long = lens.clone()
+    long[0] += 2 ** 32
+    assert torch.equal(paged_decode_attention(q, kp, vp, table, long, softcap=5.0),
+                       paged_decode_attention(q, kp, vp, table, most, softcap=5.0))
+    long[0] = 5 - 2 ** 32
+    assert not paged_decode_attention(q, kp, vp, table, long, softcap=5.0)[0].any()
+
+
+def test_long_pages_cpu():
+    _long_pages("cpu")
+
+
+@pytest.mark.gpu
+def test_long_pages_gpu():
+    _long_pages("cuda")
