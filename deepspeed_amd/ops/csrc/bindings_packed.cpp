@@ -376,6 +376,11 @@ Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
     here = here && t->device() == q_.device();
   TORCH_CHECK_VALUE(here, what, ": tensors on different devices");
   check_cap(softcap, what);
+  // keys and the steps behind the last of them are counted in 32 bits
+  constexpr int64_t KEYS = 1ll << 30;
+  TORCH_CHECK_VALUE(kpool_.size(2) <= KEYS &&
+                    table_.size(1) <= KEYS / kpool_.size(2),
+                    what, ": a table of up to 2^30 keys");
   const Opt slopes = slopes_of(alibi_slopes, q_, what);
   const OneDevice on(what, q_);
   const auto q = aligned(q_), kpool = aligned(kpool_), vpool = aligned(vpool_);
@@ -387,8 +392,7 @@ Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
   if (splits == 0) splits = shaped_splits(groups, table.size(1) * BS);
   TORCH_CHECK_VALUE(splits >= 1 && kpool.size(0) > 0 &&
                     kpool.size(0) < (1ll << 31) && H * 128 < (1ll << 31) &&
-                    n * splits * 512 < THREADS && Hkv <= 65535 &&
-                    BS < (1ll << 31) && table.size(1) < (1ll << 31),
+                    n * splits * 512 < THREADS && Hkv <= 65535,
                     what, ": size");
   const int64_t items = splits > 1 ? n * splits * Hkv * 16 : 0;
   auto part = at::empty({items * 130}, q.options().dtype(at::kFloat));

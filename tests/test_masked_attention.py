@@ -784,3 +784,18 @@ def test_long_pages_cpu():
 @pytest.mark.gpu
 def test_long_pages_gpu():
     _long_pages("cuda")
+
+
+@pytest.mark.gpu
+def test_wide_tables_gpu():
+    """Tables wider than any request, and one of more keys than are counted."""
+    q, kp, vp, table, lens = _decode_inputs([20, 32], 4, 2, 16, "cuda")
+    want = paged_decode_attention(q, kp, vp, table, lens, splits=1, softcap=5.0)
+    wide = torch.full((2, 1 << 20), -7, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    for splits in (None, 1):
+        o = paged_decode_attention(q, kp, vp, wide, lens, splits=splits, softcap=5.0)
+        torch.testing.assert_close(o.float(), want.float(), rtol=2 * BF16, atol=1e-4)
+    far = table[:, :1].expand(2, (1 << 26) + 1)
+    with pytest.raises(ValueError, match="2\\^30 keys"):
+        paged_decode_attention(q, kp, vp, far, lens, softcap=5.0)
