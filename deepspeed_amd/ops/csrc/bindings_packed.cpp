@@ -376,11 +376,13 @@ Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
     here = here && t->device() == q_.device();
   TORCH_CHECK_VALUE(here, what, ": tensors on different devices");
   check_cap(softcap, what);
-  // keys and the steps behind the last of them are counted in 32 bits
+  // keys and the steps behind the last of them are counted in 32 bits, and so are the
+  // table's blocks
   constexpr int64_t KEYS = 1ll << 30;
   TORCH_CHECK_VALUE(kpool_.size(2) <= KEYS &&
-                    table_.size(1) <= KEYS / kpool_.size(2),
-                    what, ": a table of up to 2^30 keys");
+                    table_.size(1) <= KEYS / kpool_.size(2) &&
+                    table_.numel() < 2 * KEYS,
+                    what, ": a table of up to 2^30 keys a request and 2^31 blocks");
   const Opt slopes = slopes_of(alibi_slopes, q_, what);
   const OneDevice on(what, q_);
   const auto q = aligned(q_), kpool = aligned(kpool_), vpool = aligned(vpool_);

@@ -799,3 +799,8 @@ def test_wide_tables_gpu():
     far = table[:, :1].expand(2, (1 << 26) + 1)
     with pytest.raises(ValueError, match="2\\^30 keys"):
         paged_decode_attention(q, kp, vp, far, lens, softcap=5.0)
+    many = 1 << 12
+    with pytest.raises(ValueError, match="2\\^31 blocks"):
+        paged_decode_attention(q[:1].expand(many, -1, -1), kp, vp,
+                               table[:1, :1].expand(many, 1 << 19),
+                               lens[:1].expand(many), softcap=5.0)
