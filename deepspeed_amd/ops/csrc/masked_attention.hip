@@ -29,6 +29,7 @@ namespace {
 using namespace attn;
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOWEST = -__FLT_MAX__;     // a maximum before anything was seen
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 struct View {             // element strides of [B, S, H, D]
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(
 
   // sums of the weights, and of the weights as they are rounded for the product: o is
   // over these, so that the rounding of a weight that is most of its row goes out
-  float m = -1e30f, l = 0.f, lr = 0.f;
+  float m = LOWEST, l = 0.f, lr = 0.f;
   f32x16 acc[DB] = {};
   auto fetch = [&](int k0, int buf) __attribute__((always_inline)) {
     T::template fetch<KB, TPB>(kp + k0 * a.vk.s, (int)a.vk.s, S - k0, kt[buf],
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(
                 (unsigned)width)
               p[t][r] = -__builtin_inff();
       }
-      float mt = -1e30f;
+      float mt = LOWEST;
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -293,7 +294,8 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
       }
-      const float mc = m * c;
+      // before anything was seen not infinite, which hidden scores of -inf would meet
+      const float mc = PLAIN ? fmaxf(m * c, LOWEST) : m;
       float l0 = 0.f, l1 = 0.f;
 #pragma unroll
       for (int t = 0; t < KT; ++t)

@@ -174,6 +174,8 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
   __shared__ float lds_ml[NW][NQ * 16][2];
   static_assert(16 * OSTR * 4 >= KT * D * 2, "the V tile fits");
 
+  // what a maximum begins at, and hidden scores: shaped ones are in units of log2 already
+  constexpr float LOW = SHAPED ? -__FLT_MAX__ : -1e30f;
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
   f32x4 acc[NQ][8];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    mx[n] = -1e30f;
+    mx[n] = LOW;
     l[n] = 0.f;
 #pragma unroll
     for (int d = 0; d < 8; ++d) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -323,12 +325,12 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int last = min(limit[n], key1 - 1) - kb - 4 * g;
-      float mt = -1e30f;
+      float mt = LOW;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (!whole && 16 * t + r > last) s[n][t][r] = -1e30f;
+          if (!whole && 16 * t + r > last) s[n][t][r] = LOW;
           mt = fmaxf(mt, s[n][t][r]);
         }
       mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(NW * 64, NQ == 1 ? 3 : 2) void rows_kernel(const Ar
     const int c = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
     const int rr = (tile * NQ + n) * 16 + c;
     if (rr < ncols) {
-      float mg = -1e30f, lg = 0.f, o[8] = {};
+      float mg = -__FLT_MAX__, lg = 0.f, o[8] = {};
 #pragma unroll
       for (int w = 0; w < NW; ++w) mg = fmaxf(mg, lds_ml[w][n * 16 + c][0]);
 #pragma unroll
@@ -738,7 +740,7 @@ __global__ __launch_bounds__(128) void merge_kernel(const Args a,
   if (rr >= m * G) return;      // the lanes of a column leave together
   const long long stride = (long long)a.Hkv * (16 * NQ);
   const long long at = ((long long)first * a.Hkv + hkv) * (16 * NQ) + c;
-  float mg = -1e30f;
+  float mg = -__FLT_MAX__;
   for (int i = sub; i < n; i += 32)
     mg = fmaxf(mg, a.part_ml[(at + i * stride) * 2]);
 #pragma unroll

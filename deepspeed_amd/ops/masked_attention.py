@@ -168,7 +168,9 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     then c tanh(score / c), with ``alibi_slopes`` [H] less slope times the distance of
     query and key, softmax over the keys that a query sees: those of ``rows``, or
     without them by ``causal`` all up to its own or all there are. A query that sees
-    none gives 0 and has no gradient. On a GPU bf16 and heads of 64, 96 or 128."""
+    none gives 0 and has no gradient. On a GPU bf16 and heads of 64, 96 or 128; scores and
+    a row's log of their sum are fp32 there, so that gradients lose digits with scores
+    past 1e5 and results with such past 1e9, unless a cap holds them."""
     ext = get_ext()
     if q.is_cuda and ext is not None and untransformed():
         spans, causal = (None, causal) if rows is None else (rows.spans, rows.causal)

@@ -804,3 +804,38 @@ def test_wide_tables_gpu():
         paged_decode_attention(q[:1].expand(many, -1, -1), kp, vp,
                                table[:1, :1].expand(many, 1 << 19),
                                lens[:1].expand(many), softcap=5.0)
+
+
+def _low_scores(device, kind, D):
+    """Rows whose scores are all far below 0: their softmax is that of the differences,
+    in both forms."""
+    S, H, Hk = 40, 4, 2
+    g = torch.Generator().manual_seed(21)
+    q = torch.full((1, S, H, D), 1e15).to(device, kind)
+    k = torch.full((1, S, Hk, D), -1e15).to(device, kind)
+    v = torch.randn(1, S, Hk, D, generator=g).to(device, kind)
+    n = torch.arange(1, S + 1, device=device).double()[:, None, None]
+    want = (v[0].double().cumsum(0) / n).repeat_interleave(H // Hk, 1)
+    off = v[0].double().abs().cumsum(0).repeat_interleave(H // Hk, 1) / n
+    off = (BF16 + FP32) * off + BF16 * want.abs()
+    flat = torch.zeros(H, device=device)
+    pools = [x.view(1, S // 8, 8, Hk, D)[0].transpose(1, 2).contiguous() for x in (k, v)]
+    table = torch.arange(S // 8, device=device, dtype=torch.int32)[None]
+    for how in (dict(alibi_slopes=flat), dict(softcap=9e29),
+                dict(softcap=9e29, alibi_slopes=flat)):
+        o = masked_attention(q, k, v, scale=1.0, **how)
+        assert ((o[0].double() - want).abs() <= off).all(), how
+        for length in (1, 33, S):
+            o = paged_decode_attention(q[:, 0], *pools, table, torch.tensor(
+                [length], dtype=torch.int32, device=device), scale=1.0, **how)
+            near = (o[0].double() - want[length - 1]).abs() <= off[length - 1]
+            assert near.all(), (how, length)
+
+
+def test_low_scores_cpu():
+    _low_scores("cpu", torch.float32, 128)
+
+
+@pytest.mark.gpu
+def test_low_scores_gpu():
+    _low_scores("cuda", torch.bfloat16, 128)
