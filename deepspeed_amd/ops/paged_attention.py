@@ -14,6 +14,7 @@ import torch
 
 from . import _loader
 from ._loader import get_ext
+from .linear import untransformed
 
 # Workgroups wanted in flight: four waves each, two to three to a CU of 256. More splits
 # than that only add partial results to write and merge.
@@ -101,7 +102,7 @@ def paged_decode_attention(q: torch.Tensor, kpool: torch.Tensor,
     if softcap or alibi_slopes is not None:
         if splits is not None and splits < 1:
             raise ValueError("paged_decode_attention: at least one split")
-        if q.is_cuda and ext is not None:
+        if q.is_cuda and ext is not None and untransformed():
             return ext.paged_shaped(q, kpool, vpool, block_table, lens, splits or 0,
                                     scale, softcap, alibi_slopes)
         return _torch_shaped(q, kpool, vpool, block_table, lens, scale, softcap,

@@ -839,3 +839,39 @@ def test_low_scores_cpu():
 @pytest.mark.gpu
 def test_low_scores_gpu():
     _low_scores("cuda", torch.bfloat16, 128)
+
+
+def _decode_transforms(device, kind):
+    """A tangent, a transform's gradient and a transform's batch."""
+    q, kp, vp, table, lens = _decode_inputs([20, 32], 4, 2, 16, device)
+    q, kp, vp = (x.to(kind) for x in (q, kp, vp))
+    table = table.clamp(min=0)
+    how = dict(softcap=5.0, alibi_slopes=torch.full((4,), 0.1, device=device))
+
+    def answer(q):
+        return paged_decode_attention(q, kp, vp, table, lens, **how)
+
+    o, slope = torch.func.jvp(answer, (q,), (q,))
+    grads = torch.func.grad(lambda q: answer(q).sum())(q)
+    many = torch.func.vmap(answer)(torch.stack([q, -q]))
+    return answer, q, [x.double().cpu() for x in (o, slope, grads, many)]
+
+
+def test_decode_transforms_cpu():
+    """Against differences in 64 bits."""
+    answer, q, (o, slope, grads, many) = _decode_transforms("cpu", torch.float64)
+    h = 1e-5
+    ends = [answer(q * (1 + s * h)) for s in (1, -1)]
+    torch.testing.assert_close((ends[0] - ends[1]) / (2 * h), slope, rtol=1e-6, atol=1e-8)
+    torch.testing.assert_close((grads * q).sum(), slope.sum(), rtol=1e-9, atol=1e-9)
+    assert torch.equal(o, answer(q)) and torch.equal(many[1], answer(-q))
+
+
+@pytest.mark.gpu
+def test_decode_transforms_gpu():
+    """They see the formulas, which a kernel called directly would pass by."""
+    _, _, got = _decode_transforms("cuda", torch.bfloat16)
+    _, _, want = _decode_transforms("cpu", torch.float64)
+    for x, y in zip(got, want):
+        # bf16's rounding at the end; the tangent is of sums of fp32 beside it
+        assert ((x - y).abs() <= BF16 * y.abs() + FP32 * y.abs().max()).all()
