@@ -70,15 +70,19 @@ Tensor or_none(const Opt& t) { return t.has_value() ? *t : Tensor(); }
 // The operators' autograd is here, not in Python: a backward pass of a few tens of us
 // waits as long again for the interpreter's lock in the engine's thread (a short
 // attention, there and back: 105 us so, 55 of them an empty Python function's).
-// Gradients have none of their own: a second derivative raises.
+// What has no gradient of its own says so when one is asked for.
+variable_list no_further(variable_list results, const std::string& message) {
+  if (!at::GradMode::is_enabled()) return results;
+  for (auto& t : results)
+    if (t.defined()) t = t.detach().requires_grad_(true);
+  const int64_t n = results.size();
+  auto node = std::make_shared<torch::autograd::DelayedError>(message, n);
+  return node->apply(std::move(results));
+}
+
+// Gradients: a second derivative raises.
 variable_list once(variable_list grads, const char* what) {
-  if (!at::GradMode::is_enabled()) return grads;
-  for (auto& g : grads)
-    if (g.defined()) g = g.detach().requires_grad_(true);
-  const int64_t n = grads.size();
-  auto node = std::make_shared<torch::autograd::DelayedError>(
-      std::string(what) + " is differentiable once", n);
-  return node->apply(std::move(grads));
+  return no_further(std::move(grads), std::string(what) + " is differentiable once");
 }
 
 bool wants_grad(const Tensor& t) {
@@ -407,6 +411,9 @@ Tensor paged_shaped(const Tensor& q_, const Tensor& kpool_,
       (float)(scale.has_value() ? *scale : 1.0 / std::sqrt(128.0)),
       (float)softcap, cur_stream());
   TORCH_CHECK(e == 0, what, ": launch failed, hipError_t ", e);
+  if (wants_grad(q_) || wants_grad(kpool_) || wants_grad(vpool_))
+    return no_further({o}, std::string(what) + " has no gradient on a GPU: take "
+                      "masked_attention")[0];
   return o;
 }
 

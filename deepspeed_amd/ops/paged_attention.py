@@ -97,7 +97,8 @@ def paged_decode_attention(q: torch.Tensor, kpool: torch.Tensor,
     are c tanh(score / c), with ``alibi_slopes`` [H] they are less by slope times
     the distance from the request's last token (its new one): the single-token
     form of ``masked_attention``. There a block id that is not in the pool gives
-    NaN for its request, and a length of 0 gives 0."""
+    NaN for its request, and a length of 0 gives 0; a gradient that is asked of it
+    on a GPU raises."""
     ext = get_ext()
     if softcap or alibi_slopes is not None:
         if splits is not None and splits < 1:

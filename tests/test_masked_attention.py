@@ -875,3 +875,24 @@ def test_decode_transforms_gpu():
     for x, y in zip(got, want):
         # bf16's rounding at the end; the tangent is of sums of fp32 beside it
         assert ((x - y).abs() <= BF16 * y.abs() + FP32 * y.abs().max()).all()
+
+
+@pytest.mark.gpu
+def test_decode_without_gradient_gpu():
+    """Queries or pools that need a gradient: the same answer, and a word when the
+    gradient is asked for."""
+    q, kp, vp, table, lens = _decode_inputs([20, 0, 32], 4, 2, 16, "cuda")
+    want = paged_decode_attention(q, kp, vp, table, lens, softcap=5.0)
+    assert not want.requires_grad
+    for i in range(3):
+        ins = [x.detach().requires_grad_(i == j) for j, x in enumerate((q, kp, vp))]
+        o = paged_decode_attention(*ins, table, lens, softcap=5.0)
+        assert torch.equal(o, want) and o.requires_grad
+        with pytest.raises(RuntimeError, match="no gradient on a GPU"):
+            o.float().sum().backward()
+        none = paged_decode_attention(ins[0][:0], *ins[1:], table[:0], lens[:0],
+                                      softcap=5.0)
+        assert none.shape == (0, 4, 128)
+        with torch.no_grad():
+            o = paged_decode_attention(*ins, table, lens, softcap=5.0)
+        assert torch.equal(o, want) and not o.requires_grad
