@@ -449,17 +449,19 @@ variable_list qk_norm_kernels(const Tensor& q, const Tensor& k, const Tensor& wq
     TORCH_CHECK(S <= cs.size(0), "qk_norm_rope: tables shorter than the rows");
   }
   TORCH_CHECK(tokens * 64 < THREADS && H + Hk < (1 << 24), "qk_norm_rope: size");
-  const bool back = data(dq) != nullptr || data(dk) != nullptr;
+  // (gradients of no tokens are there, but have no memory)
+  const bool back = dq.has_value();
   std::vector<long long> strides;
   auto add = [&](const at::Tensor& t, const at::Tensor& like) {
-    TORCH_CHECK(t.sizes() == like.sizes() && t.stride(3) == 1 &&
+    TORCH_CHECK(t.sizes() == like.sizes() &&
+                (t.stride(3) == 1 || t.numel() == 0) &&
                 t.scalar_type() == q.scalar_type(),
                 "qk_norm_rope: heads of one type, unit stride inside them");
     for (int d = 0; d < 3; ++d) strides.push_back(t.stride(d));
   };
   add(q, q); add(k, k);
   if (back) {
-    TORCH_CHECK(data(dq) && data(dk), "qk_norm_rope: both gradients");
+    TORCH_CHECK(dk.has_value(), "qk_norm_rope: both gradients");
     add(*dq, q); add(*dk, k);
   }
   auto yq = at::empty({B, S, H, D}, q.options());

@@ -272,3 +272,25 @@ def test_far_rows_gpu():
         there.append(y.copy_(x))
     got = _run((*there[:2], *ins[2:]), there[2:])
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def _no_tokens(device):
+    """Rows of no tokens: the weights' gradients are there, and 0."""
+    cos, sin = rope_tables(64, 8, device=device)
+    for shape in ((2, 0, 3, 64), (0, 5, 3, 64)):
+        w = [torch.ones(64, device=device, requires_grad=True) for _ in "qk"]
+        q, k = (torch.empty(shape, device=device, requires_grad=True) for _ in "qk")
+        out = qk_norm_rope(q, k, *w, cos, sin)
+        assert [x.shape for x in out] == [q.shape, k.shape]
+        grads = torch.autograd.grad(out[0].sum() + out[1].sum(), (q, k, *w))
+        assert [x.shape for x in grads] == [x.shape for x in (q, k, *w)]
+        assert not grads[2].any() and not grads[3].any()
+
+
+def test_no_tokens_cpu():
+    _no_tokens("cpu")
+
+
+@pytest.mark.gpu
+def test_no_tokens_gpu():
+    _no_tokens("cuda")
