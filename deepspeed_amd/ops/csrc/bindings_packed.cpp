@@ -588,7 +588,7 @@ struct LogitRows {
   LogitRows(const at::Tensor& x, const at::Tensor& tokens) {
     const int64_t n = x.dim();
     TORCH_CHECK(x.is_cuda() && n >= 1 && n <= 3 &&
-                (x.stride(n - 1) == 1 || x.size(n - 1) == 1),
+                (x.stride(n - 1) == 1 || x.size(n - 1) == 1 || x.numel() == 0),
                 "token_logprobs: logits [.., V], unit stride inside");
     V = x.size(n - 1);
     if (n == 3) {

@@ -464,3 +464,25 @@ def test_nan_above_infinity_cpu():
 @pytest.mark.gpu
 def test_nan_above_infinity_gpu():
     _nan_above_infinity("cuda")
+
+
+def _no_rows(device):
+    """No rows, of any strides and dimensions."""
+    for shape in ((0, 11), (2, 0, 11), (0, 3, 4, 11)):
+        x = torch.empty(*shape[:-1], 1, device=device, requires_grad=True)
+        tokens = torch.empty(shape[:-1], dtype=torch.long, device=device)
+        for top in (0, 3):
+            got = token_logprobs(x.expand(shape), tokens, top=top)
+            assert got.logprobs.shape == got.entropy.shape == tokens.shape
+            assert got.top_ids.shape == got.top_logprobs.shape == (*tokens.shape, top)
+            dx, = torch.autograd.grad(got.logprobs.sum() + got.entropy.sum(), x)
+            assert dx.shape == x.shape
+
+
+def test_no_rows_cpu():
+    _no_rows("cpu")
+
+
+@pytest.mark.gpu
+def test_no_rows_gpu():
+    _no_rows("cuda")
