@@ -228,10 +228,11 @@ struct MaskedAttention : torch::autograd::Function<MaskedAttention> {
     // the kernels take maxima of scores that a positive scale has left in order
     auto q = q_;
     double factor = 1;
-    if (!(scale > 0)) {
-      factor = scale < 0 ? -1 : scale;
+    if (!(scale >= std::numeric_limits<float>::min())) {
+      const bool flips = scale <= -std::numeric_limits<float>::min();
+      factor = flips ? -1 : scale;      // or 0, and what is as good as that in fp32
       q = q * factor;
-      scale = scale < 0 ? -scale : 1;
+      scale = flips ? -scale : 1;
     }
     q = rows_of(q);
     const auto k = rows_of(k_), v = rows_of(v_);

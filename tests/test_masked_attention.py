@@ -896,3 +896,15 @@ def test_decode_without_gradient_gpu():
         with torch.no_grad():
             o = paged_decode_attention(*ins, table, lens, softcap=5.0)
         assert torch.equal(o, want) and not o.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-37, 1e-39, 1e-46, -1e-37, -1e-39, -1e-300])
+def test_tiny_scales_gpu(scale):
+    """Scales that fp32 does not hold, or hardly, leave the mean of what is seen."""
+    q, k, v, do = _inputs(1, 70, 2, 1, 64, "cuda", seed=23)
+    at = torch.arange(70)
+    seen = (at <= at[:, None])[None].cuda()
+    for cap in (0.0, 5.0):
+        got = _grads(q, k, v, do, None, scale=scale, softcap=cap)
+        _check(got, *_reference(q, k, v, do, seen, scale, cap, None))
