@@ -4,12 +4,14 @@
 #include "bindings.h"
 
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
 #include <cmath>
 #include <limits>
 #include <tuple>
+#include <unordered_set>
 
 extern "C" int ds_packed_spans(const void* ids, int wide, const int* prefix,
                                int* spans, int B, int S, int N, int causal,
@@ -91,22 +93,45 @@ bool wants_grad(const Tensor& t) {
 
 // An eager graph that lives keeps the place of its leaves' gradients on the stream it
 // was made on. On the default one, which no capture can take in, a captured backward
-// of the same leaves ends the process: such a forward is refused.
+// of the same leaves ends the process: such a forward is refused. The leaves are mostly
+// not the inputs themselves but the weights that these come from, so they are looked for
+// through the whole graph behind the inputs, while a capture is about and only then.
 void check_capture(const char* what,
                    std::initializer_list<const Tensor*> inputs) {
+  using torch::autograd::Node;
+  const auto now =
+      c10::hip::getCurrentHIPStream((*inputs.begin())->device().index()).stream();
+  if (now == nullptr) return;            // the default stream itself
+  std::vector<const Node*> next;
+  std::vector<std::shared_ptr<Node>> held;     // of the inputs that are leaves
   for (const auto* t : inputs) {
-    if (!wants_grad(*t) || !t->is_leaf()) continue;
-    const auto place = torch::autograd::impl::try_get_grad_accumulator(*t);
-    if (!place) continue;
-    const auto kept = place->stream();
-    if (!kept || kept->id() != 0) continue;
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    const auto now = c10::hip::getCurrentHIPStream(t->device().index());
-    TORCH_CHECK(hipStreamIsCapturing(now.stream(), &status) == hipSuccess &&
-                    status == hipStreamCaptureStatusNone,
-                what, ": an eager graph of the same leaves lives, which a capture "
-                "with gradients cannot take in; end it before, or give the capture "
-                "leaves of its own");
+    if (!wants_grad(*t)) continue;
+    if (t->is_leaf()) {
+      held.push_back(torch::autograd::impl::try_get_grad_accumulator(*t));
+      if (held.back()) next.push_back(held.back().get());
+    } else {
+      next.push_back(t->grad_fn().get());
+    }
+  }
+  if (next.empty()) return;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  TORCH_CHECK(hipStreamIsCapturing(now, &status) == hipSuccess, what,
+              ": a stream of no capture status");
+  if (status == hipStreamCaptureStatusNone) return;
+  std::unordered_set<const Node*> seen(next.begin(), next.end());
+  while (!next.empty()) {
+    const Node* node = next.back();
+    next.pop_back();
+    if (dynamic_cast<const torch::autograd::AccumulateGrad*>(node)) {
+      const auto kept = const_cast<Node*>(node)->stream();
+      TORCH_CHECK(!kept || kept->id() != 0, what,
+                  ": an eager graph of the same leaves lives, which a capture with "
+                  "gradients cannot take in; end it before, or give the capture "
+                  "leaves of its own");
+    }
+    for (const auto& edge : node->next_edges())
+      if (edge.function && seen.insert(edge.function.get()).second)
+        next.push_back(edge.function.get());
   }
 }
 

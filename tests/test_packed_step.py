@@ -210,3 +210,49 @@ def test_capture_beside_an_eager_graph_gpu():
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_capture_beside_a_graph_of_the_same_weights_gpu():
+    """The same where the inputs come from weights, however far behind: refused while
+    an eager graph of these lives, sound after its end."""
+    w = torch.randn(1, 9, 4, 64, device="cuda").bfloat16().requires_grad_()
+    heads = torch.ones(64, device="cuda", dtype=torch.bfloat16)
+    cos, sin = rope_tables(64, 9, device="cuda")
+    one = torch.zeros(1, 9, 4, dtype=torch.long, device="cuda")
+    calls = [lambda x: masked_attention(x, x.detach(), x.detach()),
+             lambda x: qk_norm_rope(x.detach(), x, heads, heads, cos, sin)[1],
+             lambda x: token_logprobs(x, one).logprobs]
+    for call in calls:
+        eager = call((w * 2).exp())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = torch.zeros(3, device="cuda")
+            with pytest.raises(RuntimeError, match="eager graph"):
+                call((w * 2).exp())
+            with torch.no_grad():
+                there = call((w * 2).exp())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(there, eager) and not held.any()
+        del eager, graph, there
+
+    def step():
+        q, k = qk_norm_rope(w * 2, w.exp(), heads, heads, cos, sin)
+        got = token_logprobs(masked_attention(q, k, w.sin()), one)
+        ones = torch.ones_like(got.logprobs)
+        return torch.autograd.grad((got.logprobs, got.entropy), w, (ones, ones))[0]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(step(), want)
