@@ -48,20 +48,21 @@ struct OneDevice {
 // q, o, do [B, S, H, D], k, v [B, S, Hkv, D] with any strides between tokens
 // and heads that keep 16-byte rows: (batch, token, head) strides, in order.
 struct FlashArgs {
+  const char* what;       // the call that errors name
   int B, S, H, Hkv, D;
   std::vector<long long> strides;
   FlashArgs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-            double scale) {
+            double scale, const char* what_ = "flash") : what(what_) {
     TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() &&
                 q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
-                q.size(3) == k.size(3), "flash: q [B,S,H,D], k/v [B,S,Hkv,D]");
+                q.size(3) == k.size(3), what, ": q [B,S,H,D], k/v [B,S,Hkv,D]");
     B = q.size(0); S = q.size(1); H = q.size(2); D = q.size(3);
     Hkv = k.size(2);
-    TORCH_CHECK(D == 64 || D == 96 || D == 128, "flash: D of 64, 96 or 128");
-    TORCH_CHECK(Hkv > 0 && H % Hkv == 0, "flash: H a multiple of Hkv");
-    TORCH_CHECK(scale > 0, "flash: scale must be positive");
+    TORCH_CHECK(D == 64 || D == 96 || D == 128, what, ": D of 64, 96 or 128");
+    TORCH_CHECK(Hkv > 0 && H % Hkv == 0, what, ": H a multiple of Hkv");
+    TORCH_CHECK(scale > 0, what, ": scale must be positive");
     TORCH_CHECK(q.size(1) < (1 << 30) && q.size(0) * (int64_t)H *
-                ((S + 127) / 128) < (1ll << 31), "flash: size");
+                ((S + 127) / 128) < (1ll << 31), what, ": size");
   }
   void add(const at::Tensor& t, const at::Tensor& like) {
     TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 &&
@@ -69,7 +70,7 @@ struct FlashArgs {
                 ((uintptr_t)t.data_ptr() & 15) == 0 &&
                 t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
                 t.stride(2) % 8 == 0 && t.stride(1) >= 0 &&
-                t.stride(1) < (1 << 24), "flash: bf16 GPU, 16-byte rows");
+                t.stride(1) < (1 << 24), what, ": bf16 GPU, 16-byte rows");
     for (int d = 0; d < 3; ++d) strides.push_back(t.stride(d));
   }
 };

@@ -164,7 +164,7 @@ struct MaskedArgs : FlashArgs {
   const float* slopes = nullptr;
   MaskedArgs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
              const Opt& spans_, const Opt& slopes_, double scale, double cap)
-      : FlashArgs(q, k, v, scale) {
+      : FlashArgs(q, k, v, scale, "masked_attention") {
     TORCH_CHECK((int64_t)B * H * ((S + 127) / 128) * 256 < THREADS,
                 "masked_attention: size");
     if (data(spans_)) {

@@ -908,3 +908,12 @@ def test_tiny_scales_gpu(scale):
     for cap in (0.0, 5.0):
         got = _grads(q, k, v, do, None, scale=scale, softcap=cap)
         _check(got, *_reference(q, k, v, do, seen, scale, cap, None))
+
+
+@pytest.mark.gpu
+def test_size_refusals_gpu():
+    """Sizes that the kernels do not count are refused under the call's own name."""
+    q = torch.zeros(1, 1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    for shape in ((1, 1 << 30, 1, 64), (1 << 15, 1 << 16, 1, 64)):
+        with pytest.raises(RuntimeError, match="masked_attention: size"):
+            masked_attention(*(q.expand(shape) for _ in "qkv"))
