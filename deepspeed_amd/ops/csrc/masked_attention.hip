@@ -1010,7 +1010,8 @@ extern "C" int ds_packed_spans(const void* ids, int wide, const int* prefix,
 }
 
 // splits 0: forward (out, lse and, unless null, rest written). Else backward from out,
-// lse, rest and dout: dq, dk, dv contiguous, stat 2 B H S floats, part splits 2 B S Hkv D (or null, 1).
+// lse, rest and dout: dq, dk, dv contiguous, stat B H S floats, part splits 2 B S Hkv D
+// (or null, 1).
 // strides: (batch, token, head) of q, k, v, out, dout. cap 0: none. A hipError_t.
 extern "C" int ds_masked_attention(
     const void* q, const void* k, const void* v, void* out, float* lse,

@@ -917,3 +917,25 @@ def test_size_refusals_gpu():
     for shape in ((1, 1 << 30, 1, 64), (1 << 15, 1 << 16, 1, 64)):
         with pytest.raises(RuntimeError, match="masked_attention: size"):
             masked_attention(*(q.expand(shape) for _ in "qkv"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [150.0, 201.0, 1e4])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("heads", [(4, 2, 64), (2, 2, 96), (6, 1, 128)])
+def test_wide_caps_gpu(heads, bias, cap):
+    """Caps on either side of those that take a series near 0, with the distance bias
+    and without, heads of every size; the single token's form as well."""
+    H, Hk, D = heads
+    ids = _ids([[90, 40], [33, -7, 90]])
+    seen = _seen(ids, None, True).cuda()
+    slopes = torch.exp2(-torch.arange(1, H + 1).float()).cuda() if bias else None
+    q, k, v, do = _inputs(2, 130, H, Hk, D, "cuda", seed=25, spread=4)
+    got = _grads(q, k, v, do, packed_rows(ids.cuda()), softcap=cap, alibi_slopes=slopes)
+    _check(got, *_reference(q, k, v, do, seen, D ** -0.5, cap, slopes))
+    q, kp, vp, table, n = _decode_inputs([130, 75, 0, 700], H, Hk, 16, "cuda", spread=4)
+    for splits in (None, 1):
+        o = paged_decode_attention(q, kp, vp, table, n, splits=splits, softcap=cap,
+                                   alibi_slopes=slopes)
+        want, off = _decode_reference(q, kp, vp, table, n, 128 ** -0.5, cap, slopes)
+        assert ((o.double().cpu() - want).abs() <= off).all()
