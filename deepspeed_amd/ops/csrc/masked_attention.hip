@@ -169,6 +169,20 @@ __device__ __forceinline__ unsigned rests(float a, float b, int ab, float c,
          rest_of(c, cd << 16) << 16 | rest_of(d, cd & 0xffff0000) << 24;
 }
 
+// What rounding to the operand x left of it, as another. The scores' gradients take both:
+// those of a row add up to 0, so that dQ and dK are small beside the sums of what they
+// are made of, and with a rounding of 2^-8 they were off 64 bits by 1.41 of their own
+// rounding's 0.00166 where scores lie close together and up to 1.56 where they lie a
+// deviation of 4 apart, capped or not; with both by 1.02 to 1.12. That is 4 to 9% of a
+// training step's time. The weights are positive and add up to 1: o and dV are off by
+// 1.0 to 1.28 and by 1.28 to 1.42, and both for them too would be another 8 to 15%.
+__device__ __forceinline__ s16x8 rounded_off(const f32x16& p, int s, s16x8 x) {
+  f32x16 left;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) left[8 * s + r] = p[8 * s + r] - value(x[r]);
+  return operand(left, s);
+}
+
 // Loads into registers end here, before a loop: the compiler, which does not know of the
 // tiles' loads, would wait for these where it first uses them, in every step of the
 // loop, and so for the next tile's as well.
@@ -548,13 +562,17 @@ __global__ __launch_bounds__(256, 2) void dkdv_kernel(const Args a,
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const s16x8 pb = operand(p, s), sb = operand(dp, s);
+        const s16x8 pb = operand(p, s);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
+        for (int db = 0; db < DB; ++db)
           dva[db] =
               mfma(T::cols(dt[cur], 32 * t + 16 * s, db, ca), pb, dva[db]);
-          dka[db] =
-              mfma(T::cols(qt[cur], 32 * t + 16 * s, db, ca), sb, dka[db]);
+        const s16x8 sb = operand(dp, s), lb = rounded_off(dp, s, sb);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const s16x8 qc = T::cols(qt[cur], 32 * t + 16 * s, db, ca);
+          dka[db] = mfma(qc, sb, dka[db]);
+          dka[db] = mfma(qc, lb, dka[db]);
         }
       }
       __builtin_amdgcn_s_setprio(0);
@@ -792,22 +810,12 @@ __global__ __launch_bounds__(256, 2) void dq_kernel(const Args a,
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const s16x8 sb = operand(dp, s);
-        // of capped scores what the rounding leaves as well: without it dQ was 0.0025
-        // off 64 bits, 1.5 times its own rounding's 0.0017 (now the same), with it the
-        // pass over 1 x 8192 takes 1186 us for 1011. Without a cap 0.0024, as is dK.
-        s16x8 lb;
-        if (CAP) {
-          f32x16 left;
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            left[8 * s + r] = dp[8 * s + r] - value(sb[r]);
-          lb = operand(left, s);
-        }
+        const s16x8 lb = rounded_off(dp, s, sb);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
           const s16x8 kc = T::cols(kt[cur], 32 * t + 16 * s, db, ca);
           acc[db] = mfma(kc, sb, acc[db]);
-          if (CAP) acc[db] = mfma(kc, lb, acc[db]);
+          acc[db] = mfma(kc, lb, acc[db]);
         }
       }
     }

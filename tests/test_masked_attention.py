@@ -939,3 +939,24 @@ def test_wide_caps_gpu(heads, bias, cap):
                                    alibi_slopes=slopes)
         want, off = _decode_reference(q, kp, vp, table, n, 128 ** -0.5, cap, slopes)
         assert ((o.double().cpu() - want).abs() <= off).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("spread", [1, 4, 8])
+@pytest.mark.parametrize("heads", [(4, 1, 128), (4, 4, 64), (4, 2, 96)])
+def test_gradients_digits_gpu(heads, spread, cap):
+    """Gradients of queries and keys are off 64 bits by little more than their own
+    rounding, scores close together or far apart: scores' gradients keep 16 bits, and
+    what is left is the weights' rounding in sum(do o), which is half of a score's
+    gradient at most, sqrt(1 + 1 / 4) of the own rounding in all. A rounding of the
+    scores' gradients to bf16 would be sqrt(2) and more."""
+    H, Hk, D = heads
+    q, k, v, do = _inputs(1, 1024, H, Hk, D, "cuda", seed=3, spread=spread)
+    at = torch.arange(1024)
+    seen = (at <= at[:, None])[None].cuda()
+    got = _grads(q, k, v, do, None, softcap=cap)
+    values, _ = _reference(q, k, v, do, seen, D ** -0.5, cap, None)
+    for name, x, y in zip(("dq", "dk"), got[1:3], values[1:3]):
+        own = (y.bfloat16().double() - y).norm()
+        assert (x.double() - y).norm() <= 1.25 ** 0.5 * 1.05 * own, name
