@@ -69,13 +69,8 @@ struct Sums {
       m = t;
     }
   }
+  // an infinite logit, or one as far, has no share, where its product would be no number
   __device__ __forceinline__ void add(float x) {
-    const float d2 = (x - m) * LOG2E, e = power(d2);
-    s += e;
-    u = __builtin_fmaf(e, d2, u);
-  }
-  // an infinite logit has no share, where its product would be no number
-  __device__ __forceinline__ void add_any(float x) {
     const float d2 = (x - m) * LOG2E, e = power(d2);
     s += e;
     u = __builtin_fmaf(e, fmaxf(d2, -1e30f), u);
@@ -192,42 +187,34 @@ __global__ __launch_bounds__(CT) void rows_kernel(
   const Chunk<T>* xv = (const Chunk<T>*)(x + head);
 
   Sums a;
-  auto one = [&](float v, bool any) {
+  auto one = [&](float v) {
     a.raise(v);
-    any ? a.add_any(v) : a.add(v);
+    a.add(v);
   };
-  auto pass = [&](bool any) __attribute__((always_inline)) {
-    a = Sums();
-    for (long long j = tid; j < head; j += CT) one(ds::to_f32(x[j]), any);
-    long long j = tid;
-    for (; j + (U - 1) * CT < nv; j += U * CT) {
-      Chunk<T> v[U];
+  for (long long j = tid; j < head; j += CT) one(ds::to_f32(x[j]));
+  long long j = tid;
+  for (; j + (U - 1) * CT < nv; j += U * CT) {
+    Chunk<T> v[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) v[i] = stream(xv + j + i * CT);
-      float t = LOWEST;
+    for (int i = 0; i < U; ++i) v[i] = stream(xv + j + i * CT);
+    float t = LOWEST;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
+    for (int i = 0; i < U; ++i)
 #pragma unroll
-        for (int e = 0; e < N; ++e) t = fmaxf(t, ds::to_f32(v[i].v[e]));
-      a.raise(t);
+      for (int e = 0; e < N; ++e) t = fmaxf(t, ds::to_f32(v[i].v[e]));
+    a.raise(t);
 #pragma unroll
-      for (int i = 0; i < U; ++i)
+    for (int i = 0; i < U; ++i)
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-          any ? a.add_any(ds::to_f32(v[i].v[e])) : a.add(ds::to_f32(v[i].v[e]));
-    }
-    for (; j < nv; j += CT) {
-      const Chunk<T> v = xv[j];
+      for (int e = 0; e < N; ++e) a.add(ds::to_f32(v[i].v[e]));
+  }
+  for (; j < nv; j += CT) {
+    const Chunk<T> v = xv[j];
 #pragma unroll
-      for (int e = 0; e < N; ++e) one(ds::to_f32(v.v[e]), any);
-    }
-    for (long long k = head + nv * N + tid; k < V; k += CT)
-      one(ds::to_f32(x[k]), any);
-    join_waves(a, lds);
-  };
-  pass(false);
-  // infinite logits among others: once more, with care
-  if (a.u != a.u && a.s == a.s) pass(true);
+    for (int e = 0; e < N; ++e) one(ds::to_f32(v.v[e]));
+  }
+  for (long long k = head + nv * N + tid; k < V; k += CT) one(ds::to_f32(x[k]));
+  join_waves(a, lds);
   if (tid == 0) {
     const bool known = y >= 0 && y < V;
     finish(a, known ? ds::to_f32(x[y]) : 0.f, known, lp + row, ent + row,
@@ -346,7 +333,7 @@ __global__ __launch_bounds__(CT) void parts_kernel(
 #pragma unroll
   for (int e = 0; e < HELD; ++e) a.m = fmaxf(a.m, v[e]);
 #pragma unroll
-  for (int e = 0; e < HELD; ++e) a.add_any(v[e]);
+  for (int e = 0; e < HELD; ++e) a.add(v[e]);
   join_waves(a, lds);
   if (tid == 0) {
     float* s = sums + ((long long)row * parts + part) * 3;
