@@ -87,6 +87,13 @@ variable_list once(variable_list grads, const char* what) {
   return no_further(std::move(grads), std::string(what) + " is differentiable once");
 }
 
+// Gradients that come in: those asked for in batches have no memory of their own.
+void check_single(const variable_list& grads, const char* what) {
+  for (const auto& g : grads)
+    TORCH_CHECK(!g.defined() || g.has_storage(), what,
+                ": gradients one after another, not in batches (is_grads_batched)");
+}
+
 bool wants_grad(const Tensor& t) {
   return at::GradMode::is_enabled() && t.requires_grad();
 }
@@ -274,6 +281,7 @@ struct MaskedAttention : torch::autograd::Function<MaskedAttention> {
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_single(g, "masked_attention");
     const auto t = ctx->get_saved_variables();
     const double factor = ctx->saved_data["factor"].toDouble();
     auto [dq, dk, dv] = masked_attn_bwd(
@@ -535,6 +543,7 @@ struct QkNorm : torch::autograd::Function<QkNorm> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_single(g, "qk_norm_rope");
     const auto t = ctx->get_saved_variables();
     auto grads = once(
         qk_norm_kernels(t[0], t[1], t[2], t[3], t[4], t[5], t[6],
@@ -706,6 +715,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     return {out[0], out[1], out[3], out[4]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_single(g, "token_logprobs");
     variable_list grads(4);
     if (!g[0].defined() && !g[1].defined()) return grads;
     const auto t = ctx->get_saved_variables();

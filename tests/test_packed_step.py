@@ -256,3 +256,18 @@ def test_capture_beside_a_graph_of_the_same_weights_gpu():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want) and torch.equal(step(), want)
+
+
+@pytest.mark.gpu
+def test_gradients_in_batches_are_refused_gpu():
+    w = torch.randn(1, 9, 4, 64, device="cuda").bfloat16().requires_grad_()
+    heads = torch.ones(64, device="cuda", dtype=torch.bfloat16)
+    cos, sin = rope_tables(64, 9, device="cuda")
+    one = torch.zeros(1, 9, 4, dtype=torch.long, device="cuda")
+    for name, out in (("masked_attention", masked_attention(w, w, w)),
+                      ("qk_norm_rope", qk_norm_rope(w, w, heads, heads, cos, sin)[0]),
+                      ("token_logprobs", token_logprobs(w, one).logprobs)):
+        many = torch.stack([torch.ones_like(out)] * 2)
+        with pytest.raises(RuntimeError, match=name + ".*not in batches"):
+            torch.autograd.grad(out, w, many, is_grads_batched=True, retain_graph=True)
+        torch.autograd.grad(out, w, many[0])
