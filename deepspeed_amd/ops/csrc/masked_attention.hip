@@ -434,11 +434,12 @@ __global__ __launch_bounds__(NW * 64, KB == 32 ? 3 : 2) void fwd_kernel(
 // Both passes compute S and dP again, as attention.hip's: every sum in registers and in
 // one order, no atomics. dQ goes first and leaves sum(do * o) for the other: a kernel for
 // these alone read do once more (54 us of the nine documents' 930 in all). Bound by the
-// matrix and vector units together (39 and 57 to 65% busy; waves of two or eight to a
-// tile, a half's products beside the other half's arithmetic or prefetched operands are
-// all slower). us, cases as above: dQ 1186 (696 TFLOP/s of its three products, 4 with what
-// a rounding leaves), 313, 65, 375; dK and dV 1345 and 47 for the splits' sums (790 of
-// four), 342, 78, 365.
+// matrix and vector units together for one long document (42 to 46 and 57 to 66% busy),
+// by waves that wait for the rest of their workgroup for many (27 to 30 and 27%); waves of
+// two or eight to a tile, a half's products beside the other half's arithmetic or
+// prefetched operands are all slower. us, cases as above: dQ 1182 (930 TFLOP/s of its
+// products, four with what a rounding leaves), 345, 74, 377; dK and dV 1575 and 47 for the
+// splits' sums (873 of five), 387, 86, 414.
 //
 // dK and dV: a wave owns 32 keys and walks the queries that see them.
 template <int D, int CAP, bool BIAS>
